@@ -4,7 +4,7 @@ ARCH  ?= gfx950
 SRC   := $(wildcard vqa_amd/csrc/*.hip)
 OBJ   := $(SRC:.hip=.o)
 HDR   := $(wildcard vqa_amd/csrc/*.h) include/vqa_hip.h
-FLAGS := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -Iinclude -Ivqa_amd/csrc -Wall -Wno-unused-function
+FLAGS := --offload-arch=$(ARCH) -O3 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -Iinclude -Ivqa_amd/csrc -Wall -Wno-unused-function
 
 all: vqa_amd/libvqa_hip.so
 
