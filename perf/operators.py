@@ -272,8 +272,8 @@ def _own_scan(s):
 
 def _own_norm(s):
     from vqa_amd import ops
-    kw = dict(f=s['f'], gate=s['gate'], residual_scale=s['rho'], w_post=s['w_post'], w_pre=s['w_pre'], eps=EPS)
-    y, h, stats = ops.norm_gate_fwd(s['x'], **kw)
+    kw = dict(f=s['f'], gate=s['gate'], residual_scale=s['rho'], w_post=s['w_post'], w_pre=s['w_pre'])
+    y, h, stats = ops.norm_gate_fwd(s['x'], eps=EPS, **kw)
     if s['case']['mode'] == 'serve':
         return {'y': y, 'h': h}
     dx, df, dgate, drho, dw_post, dw_pre = ops.norm_gate_bwd(s['dy'], s['dh'], s['x'], stats, **kw)
