@@ -410,6 +410,58 @@ int vqa_colsum_rows(const void* X, int ld, float* out, const int32_t* rows, int 
 /* dst[m,0:N] = (dtype) src[m,0:N]; dst[m,N:ld_dst] = 0 */
 int vqa_cast_pad(const float* src, int ld_src, void* dst, int ld_dst, int M, int N, int dtype, hipStream_t stream);
 
+/* ---- token sequences: recurrence, cross attention, residual norms ---------------------------
+ * A block in which the tokens of a question or caption read the image: the recurrence mixes the tokens, the attention
+ * reads the regions, the norms with gate and residual update join blocks.  None has a counterpart in the reference
+ * (its question is one vector, seq2vec.py:16-25, and its image one mean, model.py:161-164).  No entry point uses
+ * atomics: the same inputs give the same bits. */
+
+/* Gated linear recurrence, the LSTM cell of vqa_lstm_cell without the recurrent product:
+ *   c_t = s(f_t) c_{t-1} + s(i_t) tanh(g_t),  h_t = s(o_t) tanh(c_t)        (s: the logistic function)
+ *   gates    (B, T) rows of 4H, gate order i, f, g, o, row (b, t) at gates + b * sb + t * st (elements, multiples of 8,
+ *            st >= 4H)
+ *   lengths  optional (B): sample b has lengths[b] steps (clamped to [0, T]); behind them the state stays, h is 0, the
+ *            gates are not read and their gradient is 0
+ *   c0       optional (B, H) fp32 starting state (0 when NULL); c_last optional (B, H) fp32: the state after the last
+ *            step, so that a call with T = 1 is one step of a running sequence
+ *   h        (B, T, H)
+ *   saved    vqa_gated_scan_saved_floats fp32 (states every VQA_GATED_SCAN_SAVE steps) for the backward; NULL when none
+ *            follows
+ *   workspace  vqa_gated_scan_workspace_floats fp32 (may be 0: NULL), scratch of one call
+ * Backward: dh (B, T, H) and dc_last (B, H) fp32, either NULL when it is zero; writes dgates (B, T, 4H) and, unless
+ * NULL, dc0 (B, H) fp32.  H % 8 == 0, T <= VQA_GATED_SCAN_MAX_T, B * H <= 2^30. */
+#define VQA_GATED_SCAN_SAVE 16
+#define VQA_GATED_SCAN_MAX_T (1 << 20)
+size_t vqa_gated_scan_workspace_floats(int B, int T, int H);
+size_t vqa_gated_scan_saved_floats(int B, int T, int H);
+int vqa_gated_scan_fwd(const void* gates, long sb, long st, const int32_t* lengths, const float* c0, void* h, float* c_last,
+                       float* saved, float* workspace, int B, int T, int H, int dtype, hipStream_t stream);
+int vqa_gated_scan_bwd(const void* dh, const float* dc_last, const void* gates, long sb, long st, const int32_t* lengths,
+                       const float* c0, const float* saved, void* dgates, float* dc0, float* workspace, int B, int T, int H,
+                       int dtype, hipStream_t stream);
+
+/* The norm behind a block, its gate, the residual update and the norm in front of the next block:
+ *   y = residual_scale * x + s(gate) * w_post * f / rms(f),   h = w_pre * y / rms(y),   rms(z) = sqrt(mean z^2 + eps)
+ *   x, f, y, h  (rows, D) of `dtype` with their leading dimensions (multiples of 8); f NULL: h = w_pre * x / rms(x)
+ *               alone (the norm in front of the first block; gate, residual_scale, w_post, y NULL too); y or h may be
+ *               NULL when it is not wanted.  h is the norm of the fp32 y, before y is rounded for storage.  y may be
+ *               x's memory and h f's.
+ *   gate        optional (rows / rows_per_gate, D) pre-activations: row r is gated by gate row r / rows_per_gate
+ *   residual_scale, w_post, w_pre  optional (D) fp32 (1 when NULL)
+ *   stats       (rows, 2) fp32: 1 / rms of f and of y, for the backward; NULL when none follows
+ * Backward: dy, dh (either NULL when zero; dy needs f); writes dx, df, dgate (as gate, summed over the rows that share it)
+ * and, unless NULL, drho (of residual_scale), dw_post, dw_pre.  workspace: vqa_norm_gate_workspace_floats (rows_per_gate 0
+ * without a gate).  D % 8 == 0, D <= 8192. */
+int vqa_norm_gate_fwd(const void* x, long ldx, const void* f, long ldf, const void* gate, long ldg, long rows_per_gate,
+                      const float* residual_scale, const float* w_post, const float* w_pre, float eps, void* y, long ldy,
+                      void* h, long ldh, float* stats, long rows, int D, int dtype, hipStream_t stream);
+size_t vqa_norm_gate_workspace_floats(long rows, int D, long rows_per_gate);
+int vqa_norm_gate_bwd(const void* dy, long lddy, const void* dh, long lddh, const void* x, long ldx, const void* f, long ldf,
+                      const void* gate, long ldg, long rows_per_gate, const float* residual_scale, const float* w_post,
+                      const float* w_pre, const float* stats, void* dx, long lddx, void* df, long lddf, void* dgate,
+                      long lddg, float* drho, float* dw_post, float* dw_pre, float* workspace, long rows, int D, int dtype,
+                      hipStream_t stream);
+
 /* ---- loss, prediction, optimiser ------------------------------------------------- */
 
 /* loss_rows[b] = logsumexp(z_b) - z_b[y_b]; dlogits = (softmax(z_b) - onehot) * grad_scale

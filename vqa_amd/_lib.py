@@ -83,15 +83,24 @@ _SIGNATURES = {
     'vqa_tanh_dropout_bwd': [_p, _i, _z, _p, _i, _p, _i, _i, _i, _u, _f, _i, _p],
     'vqa_colsum': [_p, _i, _p, _i, _i, _i, _p],
     'vqa_cast_pad': [_p, _i, _p, _i, _i, _i, _i, _p],
+    'vqa_gated_scan_workspace_floats': [_i, _i, _i],
+    'vqa_gated_scan_saved_floats': [_i, _i, _i],
+    'vqa_gated_scan_fwd': [_p, _l, _l, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
+    'vqa_gated_scan_bwd': [_p, _p, _p, _l, _l, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
+    'vqa_norm_gate_fwd': [_p, _l, _p, _l, _p, _l, _l, _p, _p, _p, _f, _p, _l, _p, _l, _p, _l, _i, _i, _p],
+    'vqa_norm_gate_workspace_floats': [_l, _i, _l],
+    'vqa_norm_gate_bwd': [_p, _l, _p, _l, _p, _l, _p, _l, _p, _l, _l, _p, _p, _p, _p, _p, _l, _p, _l, _p, _l, _p, _p, _p, _p, _l, _i, _i, _p],
     'vqa_softmax_ce': [_p, _i, _p, _p, _p, _i, _i, _i, _f, _i, _p, _p],
     'vqa_sum_scale': [_p, _p, _i, _f, _p],
     'vqa_argmax_accuracy': [_p, _i, _i, _i, _p, _p, _i, _p, _p, _p],
     'vqa_adam_step': [_p, _p, _p, _p, _p, _l, _f, _f, _f, _f, _i, _f, _p, _p],
 }
 _RESTYPE = {'vqa_last_error_string': C.c_char_p, 'vqa_attn_lds_bytes': C.c_size_t,
-            'vqa_attn_split_workspace_floats': C.c_size_t}
+            'vqa_attn_split_workspace_floats': C.c_size_t, 'vqa_gated_scan_workspace_floats': C.c_size_t,
+            'vqa_gated_scan_saved_floats': C.c_size_t, 'vqa_norm_gate_workspace_floats': C.c_size_t}
 _NO_STATUS = {'vqa_version', 'vqa_lstm_resident_workgroups', 'vqa_last_error_string', 'vqa_attn_lds_bytes', 'vqa_gemm_splitk_hint',
-              'vqa_grid_mean_splits', 'vqa_attn_splits', 'vqa_attn_split_workspace_floats'}
+              'vqa_grid_mean_splits', 'vqa_attn_splits', 'vqa_attn_split_workspace_floats',
+              'vqa_gated_scan_workspace_floats', 'vqa_gated_scan_saved_floats', 'vqa_norm_gate_workspace_floats'}
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

@@ -1,0 +1,290 @@
+"""Token-level operators of libvqa_hip.so as functions of tensors.
+
+A block in which the tokens of a question or caption read the image: ``gated_scan`` mixes the tokens,
+``cross_attention`` reads the regions, ``norm_gate`` adds a block's output to the residual stream and norms it for the
+next one.  (The reference reduces question and image to one vector each, seq2vec.py:16-25 and model.py:161-164, and has
+no counterpart.)
+
+Each operator comes as a differentiable function and as the explicit pair ``*_fwd`` / ``*_bwd`` it is made of, for
+training loops that keep their own buffers.  Tensors live on one HIP device; the work goes to torch's current stream of
+THAT device, whichever device is current.  Storage is float32 or bfloat16, arithmetic float32.  An operand whose rows
+the kernels cannot read in 16-byte pieces (odd strides or addresses) is copied first.  Outputs are new tensors.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import VqaHipError
+
+
+def _call(device, name, *args):
+    """An entry point on torch's current stream of `device`.  The stream is asked for at every call (the module's bound
+    stream belongs to the model that bound it) and the device is made current for the launch."""
+    lib = _lib.load()
+    index = device.index
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if index == torch.cuda.current_device():
+        rc = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, stream)
+    if rc != 0:
+        raise VqaHipError(f'{name} failed ({rc}): {lib.vqa_last_error_string().decode()}')
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _need(cond, msg):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _storage(name, t):
+    if t.device.type != 'cuda':
+        raise VqaHipError(f'{name} runs on a HIP device only (inputs must be cuda tensors); there is no CPU path')
+    return _lib.dtype_code(t.dtype)
+
+
+def _like(name, what, t, ref, shape, dtype=None):
+    """`t` checked against the operand `ref` it goes with."""
+    _need(tuple(t.shape) == tuple(shape), f'{name}: {what} must be {tuple(shape)}, got {tuple(t.shape)}')
+    _need(t.dtype == (dtype or ref.dtype), f'{name}: {what} must be {dtype or ref.dtype}, got {t.dtype}')
+    _need(t.device == ref.device, f'{name}: {what} is on {t.device}, the other operands on {ref.device}')
+
+
+def _packed(t):
+    """`t`, contiguous and 16-byte aligned."""
+    if t is None:
+        return None
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _lengths(name, what, t, ref, n):
+    if t is None:
+        return None
+    _need(tuple(t.shape) == (n,) and t.device == ref.device and t.dtype in (torch.int32, torch.int64),
+          f'{name}: {what} must be ({n},) int32 or int64 on {ref.device}')
+    return t.to(torch.int32).contiguous()
+
+
+# ---- gated linear recurrence -------------------------------------------------------------------
+
+def _scan_operands(gates, lengths, c0, name):
+    dt = _storage(name, gates)
+    _need(gates.dim() == 3 and gates.shape[2] % 32 == 0, f'{name}: gates must be (B, T, 4H) with H a multiple of 8')
+    B, T, H = gates.shape[0], gates.shape[1], gates.shape[2] // 4
+    sb, st, one = gates.stride()
+    if one != 1 or sb % 8 or st % 8 or (T > 1 and st < 4 * H) or sb < 0 or gates.data_ptr() % 16:
+        gates = gates.contiguous() if not gates.is_contiguous() else gates.clone()
+        sb, st, one = gates.stride()
+    st = max(st, 4 * H)
+    if c0 is not None:
+        _like(name, 'c0', c0, gates, (B, H), torch.float32)
+        c0 = _packed(c0)
+    return dt, gates, sb, st, _lengths(name, 'lengths', lengths, gates, B), c0, B, T, H
+
+
+def gated_scan_fwd(gates, lengths=None, c0=None, save=True):
+    """c_t = s(f_t) c_{t-1} + s(i_t) tanh(g_t), h_t = s(o_t) tanh(c_t) over ``gates`` (B, T, 4H), gate order i, f, g, o.
+
+    ``lengths`` (B,): steps of each sample (behind them h is 0 and the state stays); ``c0`` (B, H) float32 starting
+    state.  Returns ``h`` (B, T, H), the last state ``c`` (B, H) float32, and what ``gated_scan_bwd`` needs (None unless
+    ``save``).  With T = 1 and ``c0`` the state of the last call this is one step of a running sequence."""
+    dt, gates, sb, st, lengths, c0, B, T, H = _scan_operands(gates, lengths, c0, 'gated_scan')
+    dev = gates.device
+    h = torch.empty((B, T, H), dtype=gates.dtype, device=dev)
+    c = torch.empty((B, H), dtype=torch.float32, device=dev)
+    saved = torch.empty(((T - 1) // _SAVE if T else 0, B, H), dtype=torch.float32, device=dev) if save else None
+    if B == 0 or T == 0 or H == 0:
+        return h, c.zero_() if c0 is None else c.copy_(c0), saved
+    ws = _workspace(_lib.call('vqa_gated_scan_workspace_floats', B, T, H), dev)
+    _call(dev, 'vqa_gated_scan_fwd', gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0), h.data_ptr(), c.data_ptr(),
+          saved.data_ptr() if save and T > _SAVE else None, _ptr(ws), B, T, H, dt)
+    return h, c, saved
+
+
+def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
+    """Gradients of ``gated_scan_fwd``: (dgates (B, T, 4H), dc0 (B, H) float32) from dh (B, T, H) and dc (B, H) float32,
+    the gradient at the last state (either may be None: zero)."""
+    dt, gates, sb, st, lengths, c0, B, T, H = _scan_operands(gates, lengths, c0, 'gated_scan')
+    dev = gates.device
+    dgates = torch.empty((B, T, 4 * H), dtype=gates.dtype, device=dev)
+    dc0 = torch.empty((B, H), dtype=torch.float32, device=dev)
+    if dh is not None:
+        _like('gated_scan', 'dh', dh, gates, (B, T, H))
+        dh = _packed(dh)
+    if dc is not None:
+        _like('gated_scan', 'dc', dc, gates, (B, H), torch.float32)
+        dc = _packed(dc)
+    if B == 0 or T == 0 or H == 0 or (dh is None and dc is None):
+        return dgates.zero_(), dc0.zero_() if dc is None else dc0.copy_(dc)
+    _need(saved is not None and tuple(saved.shape) == ((T - 1) // _SAVE, B, H),
+          'gated_scan: the backward needs what gated_scan_fwd(..., save=True) returned for these gates')
+    ws = _workspace(_lib.call('vqa_gated_scan_workspace_floats', B, T, H), dev)
+    _call(dev, 'vqa_gated_scan_bwd', _ptr(dh), _ptr(dc), gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0),
+          saved.data_ptr() if T > _SAVE else None, dgates.data_ptr(), dc0.data_ptr(), _ptr(ws), B, T, H, dt)
+    return dgates, dc0
+
+
+_SAVE = 16                   # VQA_GATED_SCAN_SAVE of include/vqa_hip.h
+
+
+def _workspace(floats, device):
+    """Scratch of one call, from torch's allocator: it belongs to the stream of the call (and, under capture, to the
+    graph), so calls on two streams and two captured graphs never share it."""
+    return torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gates, lengths, c0):
+        h, c, saved = gated_scan_fwd(gates, lengths, c0, save=ctx.needs_input_grad[0] or ctx.needs_input_grad[2])
+        ctx.save_for_backward(gates, lengths, c0, saved)
+        ctx.set_materialize_grads(False)
+        return h, c
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dc):
+        gates, lengths, c0, saved = ctx.saved_tensors
+        if dh is None and dc is None:
+            return None, None, None
+        dgates, dc0 = gated_scan_bwd(dh, dc, gates, saved, lengths, c0)
+        return dgates, None, dc0 if c0 is not None else None
+
+
+def gated_scan(gates, lengths=None, c0=None):
+    """Differentiable ``gated_scan_fwd``: (h, last state)."""
+    return _GatedScan.apply(gates, lengths, c0)
+
+
+# ---- norms with gate and residual update ---------------------------------------------------------
+
+def _rows(t):
+    """(tensor, leading dimension): `t` (..., D) as rows the kernels can read, copied if its strides do not allow it."""
+    if t is None:
+        return None, 0
+    D, n = t.shape[-1], t.dim()
+    ld, ok = None, t.stride(-1) == 1 or D == 1
+    for i in range(n - 2, -1, -1):                              # one stride for all rows together
+        if t.shape[i] == 1:
+            continue
+        if ld is None:
+            ld, span = t.stride(i), t.stride(i) * t.shape[i]
+        else:
+            ok, span = ok and t.stride(i) == span, span * t.shape[i]
+    ld = D if ld is None else ld
+    if not ok or ld < D or ld % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld = D
+    return t, ld
+
+
+def _norm_operands(name, x, f, gate, residual_scale, w_post, w_pre):
+    dt = _storage(name, x)
+    _need(x.dim() >= 1 and x.shape[-1] % 8 == 0 and 8 <= x.shape[-1] <= 8192, f'{name}: the width must be a multiple of 8 in [8, 8192]')
+    D = x.shape[-1]
+    rows = x.numel() // D
+    _need(f is not None or (gate is None and residual_scale is None and w_post is None),
+          f'{name}: gate, residual_scale and w_post belong to the block output f')
+    per = 0
+    if f is not None:
+        _like(name, 'f', f, x, x.shape)
+    if gate is not None:
+        _need(gate.dtype == x.dtype and gate.device == x.device and gate.shape[-1] == D,
+              f'{name}: gate must have the width, dtype and device of x')
+        n = gate.numel() // D
+        # the gate's leading dimensions are x's up to some point, then ones: row r belongs to gate row r // per
+        lead, full = list(gate.shape[:-1]), list(x.shape[:-1])
+        _need(len(lead) <= len(full), f'{name}: gate has more dimensions than x')
+        lead += [1] * (len(full) - len(lead))
+        cut = max([i + 1 for i, s in enumerate(lead) if s != 1], default=0)
+        _need(lead[:cut] == full[:cut], f'{name}: gate {tuple(gate.shape)} must share the leading dimensions of x {tuple(x.shape)} '
+              'up to some point and have size 1 behind it')
+        per = rows // n if n else 1
+    for what, w in (('residual_scale', residual_scale), ('w_post', w_post), ('w_pre', w_pre)):
+        if w is not None:
+            _like(name, what, w, x, (D,), torch.float32)
+    return dt, D, rows, per
+
+
+def norm_gate_fwd(x, f=None, gate=None, residual_scale=None, w_post=None, w_pre=None, eps=1e-6, want_y=True, want_h=True, save=True):
+    """y = residual_scale x + s(gate) w_post f / rms(f) and h = w_pre y / rms(y) over the last dimension of ``x``.
+
+    ``gate`` holds pre-activations in x's dtype, shaped as x or with size 1 in its last leading dimensions ((B, 1, D) or
+    (B, D) for x (B, T, D): one gate row per sample); the weights are (D,) float32; what is None counts as 1.  With f
+    None only h = w_pre x / rms(x) is made.  Returns (y, h, stats): y or h None when not made, stats for
+    ``norm_gate_bwd`` (None unless ``save``)."""
+    name = 'norm_gate'
+    dt, D, rows, per = _norm_operands(name, x, f, gate, residual_scale, w_post, w_pre)
+    want_y = want_y and f is not None
+    _need(want_y or want_h, f'{name}: one of y, h must be wanted')
+    _need(want_h or w_pre is None, f'{name}: w_pre belongs to h')
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_y else None
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_h else None
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if save else None
+    if rows == 0:
+        return y, h, stats
+    (x, ldx), (f, ldf), (gate, ldg) = _rows(x), _rows(f), _rows(gate)
+    rho, w_post, w_pre = _packed(residual_scale), _packed(w_post), _packed(w_pre)
+    _call(x.device, 'vqa_norm_gate_fwd', x.data_ptr(), ldx, _ptr(f), ldf, _ptr(gate), ldg, per, _ptr(rho), _ptr(w_post), _ptr(w_pre),
+          eps, _ptr(y), D, _ptr(h), D, _ptr(stats), rows, D, dt)
+    return y, h, stats
+
+
+def norm_gate_bwd(dy, dh, x, stats, f=None, gate=None, residual_scale=None, w_post=None, w_pre=None):
+    """Gradients of ``norm_gate_fwd`` from dy and dh (either None: zero): (dx, df, dgate, dresidual_scale, dw_post,
+    dw_pre), None for what was not given (dgate in the gate's shape, summed over the rows that share a gate row)."""
+    name = 'norm_gate'
+    dt, D, rows, per = _norm_operands(name, x, f, gate, residual_scale, w_post, w_pre)
+    _need(dy is not None or dh is not None, f'{name}: one of dy, dh is needed')
+    _need(dy is None or f is not None, f'{name}: without f there is no y, so no dy')
+    for what, g in (('dy', dy), ('dh', dh)):
+        if g is not None:
+            _like(name, what, g, x, x.shape)
+    _like(name, 'stats', stats, x, (rows, 2), torch.float32)
+
+    def new(t, dtype=None):
+        return None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=x.device)
+
+    dx, df, dgate = new(x), new(f), new(gate)
+    drho, dw_post, dw_pre = new(residual_scale), new(w_post), new(w_pre)
+    if rows == 0:
+        for g in (drho, dw_post, dw_pre, dgate):
+            if g is not None:
+                g.zero_()
+        return dx, df, dgate, drho, dw_post, dw_pre
+    (x, ldx), (f, ldf), (gate, ldg), (dy, lddy), (dh, lddh) = _rows(x), _rows(f), _rows(gate), _rows(dy), _rows(dh)
+    rho, w_post, w_pre, stats = _packed(residual_scale), _packed(w_post), _packed(w_pre), _packed(stats)
+    ws = _workspace(_lib.call('vqa_norm_gate_workspace_floats', rows, D, per), x.device)
+    _call(x.device, 'vqa_norm_gate_bwd', _ptr(dy), lddy, _ptr(dh), lddh, x.data_ptr(), ldx, _ptr(f), ldf, _ptr(gate), ldg, per,
+          _ptr(rho), _ptr(w_post), _ptr(w_pre), stats.data_ptr(), dx.data_ptr(), D, _ptr(df), D, _ptr(dgate), D,
+          _ptr(drho), _ptr(dw_post), _ptr(dw_pre), ws.data_ptr(), rows, D, dt)
+    return dx, df, dgate, drho, dw_post, dw_pre
+
+
+class _NormGate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, gate, residual_scale, w_post, w_pre, eps):
+        y, h, stats = norm_gate_fwd(x, f, gate, residual_scale, w_post, w_pre, eps, save=any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, f, gate, residual_scale, w_post, w_pre, stats)
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        x, f, gate, residual_scale, w_post, w_pre, stats = ctx.saved_tensors
+        if dy is None and dh is None:
+            return (None,) * 7
+        return (*norm_gate_bwd(dy, dh, x, stats, f, gate, residual_scale, w_post, w_pre), None)
+
+
+def norm_gate(x, f=None, gate=None, residual_scale=None, w_post=None, w_pre=None, eps=1e-6):
+    """Differentiable ``norm_gate_fwd``: (y, h); y is None when f is."""
+    return _NormGate.apply(x, f, gate, residual_scale, w_post, w_pre, eps)
