@@ -49,3 +49,24 @@ def norm_gate(x, f=None, gate=None, rho=None, w_post=None, w_pre=None, eps=1e-6)
             g = torch.sigmoid(gate.reshape(*gate.shape[:-1], *(1,) * (x.dim() - gate.dim()), gate.shape[-1]))
         y = one(rho) * x + g * one(w_post) * normed(f)
     return y, one(w_pre) * normed(y)
+
+
+def attention(q, k, v, kv_len=None, mask=None, scale=None):
+    """Sample by sample over the regions that count; (o, lse)."""
+    B, Tq, H, D = q.shape
+    G = H // k.shape[2]
+    scale = D ** -0.5 if scale is None else scale
+    os, ls = [], []
+    for b in range(B):
+        idx = torch.arange(k.shape[1] if kv_len is None else max(0, min(int(kv_len[b]), k.shape[1])), device=q.device)
+        if mask is not None:
+            idx = idx[mask[b][idx].bool()]
+        if idx.numel() == 0:
+            os.append(q[b] * 0 + 0 * (k[b].sum() + v[b].sum()))      # zero, with zero gradients
+            ls.append(torch.full((H, Tq), -float('inf'), dtype=q.dtype, device=q.device))
+            continue
+        kk, vv = (x[b][idx].repeat_interleave(G, 1).transpose(0, 1) for x in (k, v))
+        z = (q[b].transpose(0, 1) @ kk.transpose(1, 2).contiguous()) * scale
+        os.append((torch.softmax(z, -1) @ vv).transpose(0, 1))
+        ls.append(torch.logsumexp(z, -1))
+    return torch.stack(os), torch.stack(ls)

@@ -1,0 +1,191 @@
+"""Cross attention against the definition in 64 bits on the same inputs, one sample after the other over the regions
+that count.
+
+fp32: a score is a sum of D <= 128 products (relative 128 x 2^-24 at worst, 1e-6 of |q||k| scale in practice) and enters an
+exponential, p is good to about 2^-21 (1 + |z|); sums over the regions keep that.  Inputs are N(0, 1), |z| < 8: outputs
+are good to 1e-5 of the largest value that is averaged (5), gradients to 1e-5 of the largest term size times the sums
+they are, stated below as 2e-5 x (sum of |terms|), computed from the 64-bit form.
+bf16: p and ds are rounded to bf16 for their products: 2^-8 of each TERM at most, so an output is good to 2^-8 x (sum of
+|terms|) where the terms are p v, p dO, ds q, ds k; o enters delta = sum dO o rounded (2^-8 of sum |dO o|), which shifts
+every ds by p times that."""
+import pytest
+import torch
+
+from _token_ref import HALF, attention, close
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(B, Tq, Tk, H, Hkv, D, dtype, seed, fused=True):
+    g = torch.Generator(device='cuda').manual_seed(seed)
+
+    def r(*s):
+        return torch.randn(*s, device='cuda', generator=g).to(dtype)
+
+    q, do = r(B, Tq, H, D), r(B, Tq, H, D)
+    if fused:
+        kv = r(B, Tk, 2, Hkv, D)
+        return q, kv[:, :, 0], kv[:, :, 1], do
+    return q, r(B, Tk, Hkv, D), r(B, Tk, Hkv, D), do
+
+
+def _bounds(q, k, v, do, o, lse, live, scale):
+    """Sums of the sizes of the terms of o, dq, dk, dv, in 64 bits (everything (B, Hkv, rows or Tk, D))."""
+    B, Tq, H, D = q.shape
+    Hkv, Tk = k.shape[2], k.shape[1]
+    G = H // Hkv
+
+    def rows(x):
+        return x.reshape(B, Tq, Hkv, G, -1).permute(0, 2, 1, 3, 4).reshape(B, Hkv, Tq * G, -1)
+
+    def back(x):
+        return x.reshape(B, Hkv, Tq, G, D).permute(0, 2, 1, 3, 4).reshape(B, Tq, H, D)
+
+    Q, DO, O = rows(q), rows(do), rows(o)
+    L = rows(lse.permute(0, 2, 1)[..., None])
+    K, V = k.transpose(1, 2), v.transpose(1, 2)
+    z = Q @ K.transpose(2, 3).contiguous() * scale
+    p = torch.where(live[:, None, None, :] & torch.isfinite(L), torch.exp(z - L), torch.zeros_like(z))
+    dp = DO @ V.transpose(2, 3).contiguous()
+    delta = (DO * O).sum(-1, keepdim=True)
+    dabs = (DO * O).abs().sum(-1, keepdim=True)
+    ds = (p * (dp - delta)).abs() + p * (DO.abs() @ V.abs().transpose(2, 3).contiguous()) * 2.0 ** -8 + p * dabs
+    pa = p
+    return (back(pa @ V.abs()), back(ds @ K.abs()) * scale, (ds.transpose(2, 3).contiguous() @ Q.abs()).transpose(1, 2) * scale,
+            (pa.transpose(2, 3).contiguous() @ DO.abs()).transpose(1, 2))
+
+
+def _run(q, k, v, do, kv_len=None, mask=None, scale=None):
+    from vqa_amd import ops
+    o, lse = ops.cross_attention_fwd(q, k, v, kv_len, mask, scale)
+    grads = ops.cross_attention_bwd(do, q, k, v, o, lse, kv_len, mask, scale)
+    return (o, lse, *grads)
+
+
+def _check(q, k, v, do, kv_len=None, mask=None, scale=None):
+    got = _run(q, k, v, do, kv_len, mask, scale)
+    B, Tk, D = q.shape[0], k.shape[1], q.shape[3]
+    live = torch.ones(B, Tk, dtype=torch.bool, device='cuda')
+    if kv_len is not None:
+        live &= torch.arange(Tk, device='cuda')[None] < kv_len[:, None]
+    if mask is not None:
+        live &= mask.bool()
+    clean = [torch.where(live[:, :, None, None], x, torch.zeros_like(x)).double() for x in (k, v)]
+    leaf = [x.requires_grad_(True) for x in (q.double(), *clean)]
+    o, lse = attention(*leaf, kv_len, mask, scale)
+    ref = torch.autograd.grad(o, leaf, do.double())
+    o, lse = o.detach(), lse.detach()
+    s = D ** -0.5 if scale is None else scale
+    lim = _bounds(*(x.detach() for x in leaf), do.double(), o, lse, live, s)
+    unit = 2e-5 if q.dtype == torch.float32 else 1.05 * HALF[torch.bfloat16]
+    fin = torch.isfinite(lse)
+    assert torch.equal(torch.isfinite(got[1]), fin)
+    assert not bool(fin.logical_not().any()) or float(got[1][~fin].max()) == -float('inf')
+    assert not bool(fin.any()) or float((got[1].double() - lse)[fin].abs().max()) <= 2e-5 * (1 + float(lse[fin].abs().max()))
+    for what, x, r, b in zip(('o', 'dq', 'dk', 'dv'), (got[0], *got[2:]), (o, *ref), lim):
+        close(x, r, unit * b + 1e-6, what)
+    dead = ~live
+    assert float(got[3][dead].abs().sum()) == 0 and float(got[4][dead].abs().sum()) == 0
+    again = _run(q, k, v, do, kv_len, mask, scale)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    return got
+
+
+SHAPES = [  # B, Tq, Tk, H, Hkv, D
+    (1, 1, 1, 1, 1, 8), (2, 1, 15, 2, 1, 16), (1, 3, 16, 4, 4, 24), (3, 2, 17, 8, 2, 40), (2, 14, 33, 3, 3, 80),
+    (2, 5, 196, 12, 4, 64), (1, 1, 700, 16, 2, 128), (2, 16, 63, 2, 2, 96), (2, 17, 65, 2, 2, 72), (1, 20, 129, 6, 3, 32),
+    (2, 33, 50, 4, 4, 56), (1, 65, 130, 8, 2, 112), (1, 130, 577, 2, 1, 128), (3, 40, 7, 4, 1, 48), (1, 8, 2000, 8, 1, 88)]
+
+
+@pytest.mark.parametrize('B,Tq,Tk,H,Hkv,D', SHAPES)
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('masked', ['none', 'len', 'mask', 'both'])
+def test_attention_and_gradients_match_64_bits(B, Tq, Tk, H, Hkv, D, dtype, masked):
+    q, k, v, do = _inputs(B, Tq, Tk, H, Hkv, D, dtype, 7 * Tk + Tq)
+    g = torch.Generator(device='cuda').manual_seed(Tk)
+    kv_len = mask = None
+    if masked in ('len', 'both'):
+        kv_len = torch.randint(0, Tk + 1, (B,), device='cuda', generator=g, dtype=torch.int32)
+    if masked in ('mask', 'both'):
+        mask = torch.rand(B, Tk, device='cuda', generator=g) < 0.6
+        if B > 1:
+            mask[0] = False                                  # a sample with nothing to attend
+    if masked != 'none':                                     # what does not count may hold anything
+        live = torch.ones(B, Tk, dtype=torch.bool, device='cuda') if mask is None else mask.clone()
+        if kv_len is not None:
+            live &= torch.arange(Tk, device='cuda')[None] < kv_len[:, None]
+        k[~live] = float('nan')
+        v[~live] = float('inf')
+    _check(q, k, v, do, kv_len, mask)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_long_and_many(dtype):
+    """Key ranges split over workgroups (few rows, many regions) and many row blocks."""
+    for B, Tq, Tk, H, Hkv, D in ((1, 1, 4096, 8, 2, 64), (2, 4, 3001, 4, 1, 128), (1, 300, 1111, 4, 2, 64)):
+        q, k, v, do = _inputs(B, Tq, Tk, H, Hkv, D, dtype, Tk)
+        _check(q, k, v, do)
+        _check(q, k, v, do, kv_len=torch.full((B,), Tk // 3, device='cuda', dtype=torch.int32))
+
+
+def test_strides_scale_and_sharp_scores():
+    q, k, v, do = _inputs(2, 6, 37, 4, 2, 32, torch.bfloat16, 1, fused=False)
+    want = _check(q, k, v, do, scale=0.3)
+    heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]        # (B, H, T, D) storage
+    for a, b in zip(want, _run(*heads_first, do.transpose(1, 2).contiguous().transpose(1, 2), scale=0.3)):
+        assert torch.equal(a, b)
+    odd = [torch.empty(x.numel() + 1, device='cuda', dtype=x.dtype)[1:].view(x.shape).copy_(x) for x in (q, k, v, do)]
+    for a, b in zip(want, _run(*odd, scale=0.3)):
+        assert torch.equal(a, b)
+    one = [k[:, :, :1].expand(-1, -1, 2, -1), v[:, :1].expand(-1, 37, -1, -1)]               # stride 0: broadcast keys
+    for a, b in zip(_run(q, *one, do), _run(q, *(x.contiguous() for x in one), do)):
+        assert torch.equal(a, b)
+    # one region far above the others, in a late tile: the running maximum jumps
+    q, k, v, do = _inputs(1, 20, 300, 2, 2, 64, torch.float32, 2, fused=False)
+    k[:, 271] = 6 * q[:, 3]
+    _check(q, k, v, do)
+
+
+def test_infinite_and_nan_operands_spread_as_in_the_formula():
+    from vqa_amd import ops
+    q, k, v, do = _inputs(2, 3, 40, 2, 2, 16, torch.float32, 3, fused=False)
+    v[0, 5, 0, 2] = float('nan')
+    k[1, 7, 1, 0] = float('nan')
+    o, _ = ops.cross_attention_fwd(q, k, v)
+    bad = torch.isnan(o)
+    want = torch.zeros_like(bad)
+    want[0, :, 0, 2] = True
+    want[1, :, 1] = True
+    assert torch.equal(bad, want)
+
+
+def test_gradient_against_differences():
+    """Central differences of the fp32 forward, step 1e-2: truncation 1e-4 of the gradient's norm, noise (o good to 1e-6,
+    n random terms) / (2 step) about 1e-4 of it."""
+    from vqa_amd import ops
+    q, k, v, do = _inputs(2, 7, 45, 4, 2, 32, torch.float32, 4, fused=False)
+    kv_len = torch.tensor([45, 30], device='cuda')
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+
+    def loss(x):
+        return (ops.cross_attention(*x, kv_len=kv_len).double() * do.double()).sum()
+
+    grads = torch.autograd.grad(loss(leaves), leaves)
+    g = torch.Generator(device='cuda').manual_seed(5)
+    with torch.no_grad():
+        for i in range(3):
+            d = torch.randn(leaves[i].shape, device='cuda', generator=g)
+            up, dn = [x.detach() for x in leaves], [x.detach() for x in leaves]
+            up[i], dn[i] = up[i] + 1e-2 * d, dn[i] - 1e-2 * d
+            num, ana = float((loss(up) - loss(dn)) / 2e-2), float((grads[i].double() * d.double()).sum())
+            assert abs(num - ana) <= 5e-3 * float(grads[i].norm()), (i, num, ana)
+
+
+def test_empty_sizes():
+    from vqa_amd import ops
+    for B, Tq, Tk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        q, k = torch.randn(B, Tq, 2, 8, device='cuda'), torch.randn(B, Tk, 1, 8, device='cuda')
+        o, lse = ops.cross_attention_fwd(q, k, k)
+        assert o.shape == q.shape and float(o.abs().sum()) == 0 and lse.shape == (B, 2, Tq)
+        dq, dk, dv = ops.cross_attention_bwd(o, q, k, k, o, lse)
+        assert dq.shape == q.shape and dk.shape == k.shape and float(dq.abs().sum() + dk.abs().sum() + dv.abs().sum()) == 0

@@ -87,6 +87,10 @@ _SIGNATURES = {
     'vqa_gated_scan_saved_floats': [_i, _i, _i],
     'vqa_gated_scan_fwd': [_p, _l, _l, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     'vqa_gated_scan_bwd': [_p, _p, _p, _l, _l, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
+    'vqa_cross_attn_fwd_workspace_floats': [_i, _i, _i, _i, _i, _i, _i],
+    'vqa_cross_attn_bwd_workspace_floats': [_i, _i, _i, _i, _i, _i, _i],
+    'vqa_cross_attn_fwd': [_p, _p, _p, _p, _p, _l, _f, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
+    'vqa_cross_attn_bwd': [_p, _p, _p, _p, _p, _p, _p, _p, _l, _f, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
     'vqa_norm_gate_fwd': [_p, _l, _p, _l, _p, _l, _l, _p, _p, _p, _f, _p, _l, _p, _l, _p, _l, _i, _i, _p],
     'vqa_norm_gate_workspace_floats': [_l, _i, _l],
     'vqa_norm_gate_bwd': [_p, _l, _p, _l, _p, _l, _p, _l, _p, _l, _l, _p, _p, _p, _p, _p, _l, _p, _l, _p, _l, _p, _p, _p, _p, _l, _i, _i, _p],
@@ -97,10 +101,12 @@ _SIGNATURES = {
 }
 _RESTYPE = {'vqa_last_error_string': C.c_char_p, 'vqa_attn_lds_bytes': C.c_size_t,
             'vqa_attn_split_workspace_floats': C.c_size_t, 'vqa_gated_scan_workspace_floats': C.c_size_t,
-            'vqa_gated_scan_saved_floats': C.c_size_t, 'vqa_norm_gate_workspace_floats': C.c_size_t}
+            'vqa_gated_scan_saved_floats': C.c_size_t, 'vqa_norm_gate_workspace_floats': C.c_size_t,
+            'vqa_cross_attn_fwd_workspace_floats': C.c_size_t, 'vqa_cross_attn_bwd_workspace_floats': C.c_size_t}
 _NO_STATUS = {'vqa_version', 'vqa_lstm_resident_workgroups', 'vqa_last_error_string', 'vqa_attn_lds_bytes', 'vqa_gemm_splitk_hint',
               'vqa_grid_mean_splits', 'vqa_attn_splits', 'vqa_attn_split_workspace_floats',
-              'vqa_gated_scan_workspace_floats', 'vqa_gated_scan_saved_floats', 'vqa_norm_gate_workspace_floats'}
+              'vqa_gated_scan_workspace_floats', 'vqa_gated_scan_saved_floats', 'vqa_norm_gate_workspace_floats',
+              'vqa_cross_attn_fwd_workspace_floats', 'vqa_cross_attn_bwd_workspace_floats'}
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
@@ -160,6 +166,11 @@ def call(name: str, *args):
     if rc != 0:
         raise VqaHipError(f'{name} failed ({rc}): {lib.vqa_last_error_string().decode()}')
     return rc
+
+
+class AttnView(C.Structure):
+    """VqaAttnView of include/vqa_hip.h."""
+    _fields_ = [('data', C.c_void_p), ('sb', C.c_long), ('st', C.c_long), ('sh', C.c_long)]
 
 
 class ColsumDesc(C.Structure):

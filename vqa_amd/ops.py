@@ -12,6 +12,8 @@ the kernels cannot read in 16-byte pieces (odd strides or addresses) is copied f
 """
 from __future__ import annotations
 
+from ctypes import byref
+
 import torch
 
 from . import _lib
@@ -288,3 +290,93 @@ class _NormGate(torch.autograd.Function):
 def norm_gate(x, f=None, gate=None, residual_scale=None, w_post=None, w_pre=None, eps=1e-6):
     """Differentiable ``norm_gate_fwd``: (y, h); y is None when f is."""
     return _NormGate.apply(x, f, gate, residual_scale, w_post, w_pre, eps)
+
+
+# ---- cross attention -----------------------------------------------------------------------------
+
+def _view(t):
+    """(tensor, VqaAttnView) of a (B, T, H, D) operand, copied if the kernels cannot read its strides."""
+    st = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+    if (t.stride(3) != 1 and t.shape[3] != 1) or any(s % 8 or s < 0 for s in st[:3]) or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = t.stride()
+    return t, _lib.AttnView(t.data_ptr(), st[0], st[1], st[2])
+
+
+def _attn_operands(q, k, v, kv_len, mask, scale):
+    name = 'cross_attention'
+    dt = _storage(name, q)
+    _need(q.dim() == 4 and k.dim() == 4, f'{name}: q is (B, Tq, H, D), k and v are (B, Tk, Hkv, D)')
+    B, Tq, H, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    _like(name, 'k', k, q, (B, Tk, Hkv, D))
+    _like(name, 'v', v, q, (B, Tk, Hkv, D))
+    _need(Hkv > 0 and H > 0 and H % Hkv == 0, f'{name}: {H} query heads cannot share {Hkv} key heads evenly')
+    _need(D % 8 == 0 and 8 <= D <= 128, f'{name}: the head width must be a multiple of 8 in [8, 128], got {D}')
+    mask_sb = 0
+    if mask is not None:
+        _need(tuple(mask.shape) == (B, Tk) and mask.device == q.device and mask.dtype in (torch.bool, torch.uint8),
+              f'{name}: mask must be ({B}, {Tk}) bool or uint8 on {q.device}')
+        if (Tk > 1 and mask.stride(1) != 1) or mask.stride(0) < 0:
+            mask = mask.contiguous()
+        mask_sb = mask.stride(0)
+    return dt, _lengths(name, 'kv_len', kv_len, q, B), mask, mask_sb, D ** -0.5 if scale is None else float(scale), B, Tq, Tk, H, Hkv, D
+
+
+def cross_attention_fwd(q, k, v, kv_len=None, mask=None, scale=None):
+    """softmax(scale q k^T) v of the token rows ``q`` (B, Tq, H, D) over the regions ``k``, ``v`` (B, Tk, Hkv, D); head h
+    reads key head h // (H // Hkv).
+
+    ``kv_len`` (B,): regions of each sample; ``mask`` (B, Tk): regions that count (True); what does not count is not
+    read.  ``scale`` defaults to D ** -0.5.  Returns o (B, Tq, H, D) and the log-sum-exp (B, H, Tq) float32 that
+    ``cross_attention_bwd`` needs; a row with nothing to attend gives 0 and -inf."""
+    dt, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D = _attn_operands(q, k, v, kv_len, mask, scale)
+    dev = q.device
+    o = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
+    if B == 0 or Tq == 0 or Tk == 0:
+        return o.zero_(), lse.fill_(float('-inf'))
+    (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
+    ws = _workspace(_lib.call('vqa_cross_attn_fwd_workspace_floats', B, Tq, Tk, H, Hkv, D, dt), dev)
+    _call(dev, 'vqa_cross_attn_fwd', byref(vq), byref(vk), byref(vv), _ptr(kv_len), _ptr(mask), mask_sb, scale, o.data_ptr(),
+          lse.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
+    return o, lse
+
+
+def cross_attention_bwd(do, q, k, v, o, lse, kv_len=None, mask=None, scale=None):
+    """Gradients (dq, dk, dv) of ``cross_attention_fwd`` from do (B, Tq, H, D) and what it returned."""
+    dt, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D = _attn_operands(q, k, v, kv_len, mask, scale)
+    dev = q.device
+    _like('cross_attention', 'do', do, q, q.shape)
+    _like('cross_attention', 'o', o, q, q.shape)
+    _like('cross_attention', 'lse', lse, q, (B, H, Tq), torch.float32)
+    dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
+    dk, dv = (torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=dev) for _ in range(2))
+    if B == 0 or Tq == 0 or Tk == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
+    do, o, lse = _packed(do), _packed(o), _packed(lse)
+    ws = _workspace(_lib.call('vqa_cross_attn_bwd_workspace_floats', B, Tq, Tk, H, Hkv, D, dt), dev)
+    _call(dev, 'vqa_cross_attn_bwd', do.data_ptr(), byref(vq), byref(vk), byref(vv), o.data_ptr(), lse.data_ptr(), _ptr(kv_len),
+          _ptr(mask), mask_sb, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
+    return dq, dk, dv
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, kv_len, mask, scale):
+        o, lse = cross_attention_fwd(q, k, v, kv_len, mask, scale)
+        ctx.save_for_backward(q, k, v, o, lse, kv_len, mask)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, kv_len, mask = ctx.saved_tensors
+        return (*cross_attention_bwd(do, q, k, v, o, lse, kv_len, mask, ctx.scale), None, None, None)
+
+
+def cross_attention(q, k, v, kv_len=None, mask=None, scale=None):
+    """Differentiable ``cross_attention_fwd``: o alone."""
+    return _CrossAttention.apply(q, k, v, kv_len, mask, scale)
