@@ -430,7 +430,7 @@ int vqa_cast_pad(const float* src, int ld_src, void* dst, int ld_dst, int M, int
  *   workspace  vqa_gated_scan_workspace_floats fp32 (may be 0: NULL), scratch of one call
  * Backward: dh (B, T, H) and dc_last (B, H) fp32, either NULL when it is zero; writes dgates (B, T, 4H) and, unless
  * NULL, dc0 (B, H) fp32.  H % 8 == 0, T <= VQA_GATED_SCAN_MAX_T, B * H <= 2^30. */
-#define VQA_GATED_SCAN_SAVE 16
+#define VQA_GATED_SCAN_SAVE 8
 #define VQA_GATED_SCAN_MAX_T (1 << 20)
 size_t vqa_gated_scan_workspace_floats(int B, int T, int H);
 size_t vqa_gated_scan_saved_floats(int B, int T, int H);
@@ -477,7 +477,7 @@ int vqa_cross_attn_bwd(const void* d_o, const VqaAttnView* q, const VqaAttnView*
  *   stats       (rows, 2) fp32: 1 / rms of f and of y, for the backward; NULL when none follows
  * Backward: dy, dh (either NULL when zero; dy needs f); writes dx, df, dgate (as gate, summed over the rows that share it)
  * and, unless NULL, drho (of residual_scale), dw_post, dw_pre.  workspace: vqa_norm_gate_workspace_floats (rows_per_gate 0
- * without a gate).  D % 8 == 0, D <= 8192. */
+ * without a gate).  D % 8 == 0, D <= 8192, at most 2^30 rows. */
 int vqa_norm_gate_fwd(const void* x, long ldx, const void* f, long ldf, const void* gate, long ldg, long rows_per_gate,
                       const float* residual_scale, const float* w_post, const float* w_pre, float eps, void* y, long ldy,
                       void* h, long ldh, float* stats, long rows, int D, int dtype, hipStream_t stream);

@@ -14,6 +14,12 @@ namespace {
 constexpr int SAVE = VQA_GATED_SCAN_SAVE;       // the forward saves the state every SAVE steps; the backward recomputes between
 constexpr int BLK = 4;                          // steps whose loads a thread of the forward has in flight
 
+// The hardware's exp2 and reciprocal, 1 ulp each (a division, or the library's exponential, would cost several times as
+// many instructions): s(x) is good to 2^-22 relative, tanh x = 1 - 2 / (1 + e^2x) to 2^-22 absolute; both reach their
+// limits without overflow (1 / inf = 0).
+__device__ __forceinline__ float sigm(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
+__device__ __forceinline__ float tanh_(float x) { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.8853900817779268f * x)); }
+
 // V neighbouring values in storage form
 template <typename T, int V> struct Raw;
 template <> struct Raw<bf16_t, 4> { u16x4 r; };
@@ -75,17 +81,19 @@ __global__ void __launch_bounds__(256) k_scan_fwd(Args<T> a) {
     T* h = a.h + ((size_t)b * a.T_) * a.H + u;
     constexpr int NG = SUMMARY ? 3 : 4;
     Raw<T, V> cur[BLK][NG], nxt[BLK][NG];
-    auto fetch = [&](Raw<T, V> (&r)[BLK][NG], int t) {
+    auto fetch = [&](int t) {                                // steps past the end request the last one again: no branches
 #pragma unroll
         for (int j = 0; j < BLK; ++j)
-            if (t + j < live) {
 #pragma unroll
-                for (int q = 0; q < NG; ++q) r[j][q] = load_raw<T, V>(g + (size_t)(t + j) * a.st + (size_t)q * a.H);
-            }
+            for (int q = 0; q < NG; ++q) nxt[j][q] = load_raw<T, V>(g + (size_t)min(t + j, live - 1) * a.st + (size_t)q * a.H);
     };
-    fetch(cur, t0);
+    if (t0 < live) fetch(t0);
     for (int t = t0; t < live; t += BLK) {
-        fetch(nxt, t + BLK);
+#pragma unroll
+        for (int j = 0; j < BLK; ++j)
+#pragma unroll
+            for (int q = 0; q < NG; ++q) cur[j][q] = nxt[j][q];
+        if (t + BLK < live) fetch(t + BLK);
 #pragma unroll
         for (int j = 0; j < BLK; ++j) {
             if (t + j < live) {
@@ -96,18 +104,14 @@ __global__ void __launch_bounds__(256) k_scan_fwd(Args<T> a) {
                 float hv[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float f = fast_sigmoid(value(cur[j][1], i));
-                    c[i] = f * c[i] + fast_sigmoid(value(cur[j][0], i)) * fast_tanh(value(cur[j][2], i));
+                    const float f = sigm(value(cur[j][1], i));
+                    c[i] = f * c[i] + sigm(value(cur[j][0], i)) * tanh_(value(cur[j][2], i));
                     if (SUMMARY) P[i] *= f;
-                    else hv[i] = fast_sigmoid(value(cur[j][NG - 1], i)) * fast_tanh(c[i]);
+                    else hv[i] = sigm(value(cur[j][NG - 1], i)) * tanh_(c[i]);
                 }
                 if (!SUMMARY) store_values<T, V>(h + (size_t)(t + j) * a.H, hv);
             }
         }
-#pragma unroll
-        for (int j = 0; j < BLK; ++j)
-#pragma unroll
-            for (int q = 0; q < NG; ++q) cur[j][q] = nxt[j][q];
     }
     if (SUMMARY) {
 #pragma unroll
@@ -198,28 +202,38 @@ __global__ void __launch_bounds__(256) k_scan_bwd(Args<T> a) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) store_values<T, V>(dg + ((size_t)t * 4 + q) * a.H, zero);
     }
-    for (int s0 = live > t0 ? (live - 1) / SAVE * SAVE : t0 - SAVE; s0 >= t0; s0 -= SAVE) {
-        const int n = min(SAVE, live - s0);
-        Raw<T, V> r[SAVE][4], d[SAVE];
+    struct { Raw<T, V> r[SAVE][4], d[SAVE]; float c[V]; } cur, nxt;
+    auto fetch = [&](int s0) {
 #pragma unroll
-        for (int j = 0; j < SAVE; ++j)
-            if (j < n) {
+        for (int j = 0; j < SAVE; ++j) {
+            const size_t t = min(s0 + j, live - 1);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) r[j][q] = load_raw<T, V>(g + (size_t)(s0 + j) * a.st + (size_t)q * a.H);
-                if (dh) d[j] = load_raw<T, V>(dh + (size_t)(s0 + j) * a.H);
-            }
-        float c[SAVE + 1][V];                                // c[j]: the state before step s0 + j
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (s0 > 0) c[0][i] = a.saved[(s0 / SAVE - 1) * plane + su + i];
-            else c[0][i] = a.c0 ? a.c0[su + i] : 0.f;
+            for (int q = 0; q < 4; ++q) nxt.r[j][q] = load_raw<T, V>(g + t * a.st + (size_t)q * a.H);
+            if (dh) nxt.d[j] = load_raw<T, V>(dh + t * a.H);
         }
 #pragma unroll
-        for (int j = 0; j < SAVE; ++j)
-            if (j < n) {
+        for (int i = 0; i < V; ++i) {
+            if (s0 > 0) nxt.c[i] = a.saved[(s0 / SAVE - 1) * plane + su + i];
+            else nxt.c[i] = a.c0 ? a.c0[su + i] : 0.f;
+        }
+    };
+    const int s_last = live > t0 ? (live - 1) / SAVE * SAVE : t0 - SAVE;
+    if (live > t0) fetch(s_last);
+    for (int s0 = s_last; s0 >= t0; s0 -= SAVE) {
+        cur = nxt;
+        if (s0 > t0) fetch(s0 - SAVE);
+        const int n = live - s0;
+        float c[SAVE + 1][V], act[SAVE][3][V];               // c[j]: the state before step s0 + j
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    c[j + 1][i] = fast_sigmoid(value(r[j][1], i)) * c[j][i] + fast_sigmoid(value(r[j][0], i)) * fast_tanh(value(r[j][2], i));
+        for (int i = 0; i < V; ++i) c[0][i] = cur.c[i];
+#pragma unroll
+        for (int j = 0; j < SAVE; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {                    // (steps past the end: computed from the last one's gates, not used)
+                act[j][0][i] = sigm(value(cur.r[j][0], i));
+                act[j][1][i] = sigm(value(cur.r[j][1], i));
+                act[j][2][i] = tanh_(value(cur.r[j][2], i));
+                c[j + 1][i] = act[j][1][i] * c[j][i] + act[j][0][i] * act[j][2][i];
             }
 #pragma unroll
         for (int j = SAVE - 1; j >= 0; --j)
@@ -227,9 +241,8 @@ __global__ void __launch_bounds__(256) k_scan_bwd(Args<T> a) {
                 float o4[4][V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float si = fast_sigmoid(value(r[j][0], i)), sf = fast_sigmoid(value(r[j][1], i));
-                    const float tg = fast_tanh(value(r[j][2], i)), so = fast_sigmoid(value(r[j][3], i));
-                    const float tc = fast_tanh(c[j + 1][i]), e = dh ? value(d[j], i) : 0.f;
+                    const float si = act[j][0][i], sf = act[j][1][i], tg = act[j][2][i], so = sigm(value(cur.r[j][3], i));
+                    const float tc = tanh_(c[j + 1][i]), e = dh ? value(cur.d[j], i) : 0.f;
                     const float dct = e * so * (1.f - tc * tc) + dc[i];
                     o4[0][i] = dct * tg * si * (1.f - si);
                     o4[1][i] = dct * c[j][i] * sf * (1.f - sf);
@@ -254,14 +267,14 @@ __global__ void __launch_bounds__(256) k_scan_bwd(Args<T> a) {
 }
 
 // Chunks: one when the (sample, unit) pairs alone give every CU work or the sequence is short; otherwise as many as make
-// about 2048 waves, at least 2 SAVE steps each.  A multiple of SAVE, so that a chunk starts at a saved state.
+// about 2048 waves, at least 4 SAVE steps each.  A multiple of SAVE, so that a chunk starts at a saved state.
 int chunk_of(int B, int T_, int H) {
     const long waves = ((long)B * H / 4 + 63) / 64;
-    if (waves >= 1024 || T_ <= 4 * SAVE) return (T_ + SAVE - 1) / SAVE * SAVE;
+    if (waves >= 1024 || T_ <= 8 * SAVE) return (T_ + SAVE - 1) / SAVE * SAVE;
     const long n = (2048 + waves - 1) / waves;
     long c = (T_ + n - 1) / n;
     c = (c + SAVE - 1) / SAVE * SAVE;
-    return (int)(c < 2 * SAVE ? 2 * SAVE : c);
+    return (int)(c < 4 * SAVE ? 4 * SAVE : c);
 }
 int chunks_of(int B, int T_, int H) { const int c = chunk_of(B, T_, H); return (T_ + c - 1) / c; }
 

@@ -133,7 +133,7 @@ def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
     return dgates, dc0
 
 
-_SAVE = 16                   # VQA_GATED_SCAN_SAVE of include/vqa_hip.h
+_SAVE = 8                    # VQA_GATED_SCAN_SAVE of include/vqa_hip.h
 
 
 def _workspace(floats, device):
