@@ -12,6 +12,7 @@ the kernels cannot read in 16-byte pieces (odd strides or addresses) is copied f
 """
 from __future__ import annotations
 
+import functools
 from ctypes import byref
 
 import torch
@@ -23,38 +24,48 @@ from ._lib import VqaHipError
 def _call(device, name, *args):
     """An entry point on torch's current stream of `device`.  The stream is asked for at every call (the module's bound
     stream belongs to the model that bound it) and the device is made current for the launch."""
-    lib = _lib.load()
-    index = device.index
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if index == torch.cuda.current_device():
-        rc = getattr(lib, name)(*args, stream)
+    fn = _entry(name)
+    stream = _raw_stream(device.index)
+    if device.index == _current_device():
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, stream)
+            rc = fn(*args, stream)
     if rc != 0:
-        raise VqaHipError(f'{name} failed ({rc}): {lib.vqa_last_error_string().decode()}')
+        raise VqaHipError(f'{name} failed ({rc}): {_lib.load().vqa_last_error_string().decode()}')
+
+
+# handle of torch's current stream of a device, and the current device, without the Python objects around them: a
+# microsecond each on calls whose kernels take three
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
+
+
+@functools.lru_cache(None)
+def _entry(name):
+    return getattr(_lib.load(), name)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _need(cond, msg):
+def _need(cond, msg, *args):
     if not cond:
-        raise ValueError(msg)
+        raise ValueError(msg.format(*args))
 
 
 def _storage(name, t):
-    if t.device.type != 'cuda':
+    if not t.is_cuda:
         raise VqaHipError(f'{name} runs on a HIP device only (inputs must be cuda tensors); there is no CPU path')
     return _lib.dtype_code(t.dtype)
 
 
 def _like(name, what, t, ref, shape, dtype=None):
     """`t` checked against the operand `ref` it goes with."""
-    _need(tuple(t.shape) == tuple(shape), f'{name}: {what} must be {tuple(shape)}, got {tuple(t.shape)}')
-    _need(t.dtype == (dtype or ref.dtype), f'{name}: {what} must be {dtype or ref.dtype}, got {t.dtype}')
-    _need(t.device == ref.device, f'{name}: {what} is on {t.device}, the other operands on {ref.device}')
+    if t.shape != shape or t.dtype != (dtype or ref.dtype) or t.device != ref.device:
+        raise ValueError(f'{name}: {what} must be {tuple(shape)} {dtype or ref.dtype} on {ref.device}, '
+                         f'got {tuple(t.shape)} {t.dtype} on {t.device}')
 
 
 def _packed(t):
@@ -69,16 +80,18 @@ def _packed(t):
 def _lengths(name, what, t, ref, n):
     if t is None:
         return None
-    _need(tuple(t.shape) == (n,) and t.device == ref.device and t.dtype in (torch.int32, torch.int64),
-          f'{name}: {what} must be ({n},) int32 or int64 on {ref.device}')
-    return t.to(torch.int32).contiguous()
+    _need(t.shape == (n,) and t.device == ref.device and t.dtype in (torch.int32, torch.int64),
+          '{}: {} must be ({},) int32 or int64 on {}', name, what, n, ref.device)
+    if t.dtype != torch.int32:
+        t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
 
 
 # ---- gated linear recurrence -------------------------------------------------------------------
 
 def _scan_operands(gates, lengths, c0, name):
     dt = _storage(name, gates)
-    _need(gates.dim() == 3 and gates.shape[2] % 32 == 0, f'{name}: gates must be (B, T, 4H) with H a multiple of 8')
+    _need(gates.dim() == 3 and gates.shape[2] % 32 == 0, '{}: gates must be (B, T, 4H) with H a multiple of 8', name)
     B, T, H = gates.shape[0], gates.shape[1], gates.shape[2] // 4
     sb, st, one = gates.stride()
     if one != 1 or sb % 8 or st % 8 or (T > 1 and st < 4 * H) or sb < 0 or gates.data_ptr() % 16:
@@ -104,7 +117,7 @@ def gated_scan_fwd(gates, lengths=None, c0=None, save=True):
     saved = torch.empty(((T - 1) // _SAVE if T else 0, B, H), dtype=torch.float32, device=dev) if save else None
     if B == 0 or T == 0 or H == 0:
         return h, c.zero_() if c0 is None else c.copy_(c0), saved
-    ws = _workspace(_lib.call('vqa_gated_scan_workspace_floats', B, T, H), dev)
+    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H), dev)
     _call(dev, 'vqa_gated_scan_fwd', gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0), h.data_ptr(), c.data_ptr(),
           saved.data_ptr() if save and T > _SAVE else None, _ptr(ws), B, T, H, dt)
     return h, c, saved
@@ -127,7 +140,7 @@ def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
         return dgates.zero_(), dc0.zero_() if dc is None else dc0.copy_(dc)
     _need(saved is not None and tuple(saved.shape) == ((T - 1) // _SAVE, B, H),
           'gated_scan: the backward needs what gated_scan_fwd(..., save=True) returned for these gates')
-    ws = _workspace(_lib.call('vqa_gated_scan_workspace_floats', B, T, H), dev)
+    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H), dev)
     _call(dev, 'vqa_gated_scan_bwd', _ptr(dh), _ptr(dc), gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0),
           saved.data_ptr() if T > _SAVE else None, dgates.data_ptr(), dc0.data_ptr(), _ptr(ws), B, T, H, dt)
     return dgates, dc0
@@ -172,6 +185,8 @@ def _rows(t):
     if t is None:
         return None, 0
     D, n = t.shape[-1], t.dim()
+    if t.is_contiguous():
+        return (t if t.data_ptr() % 16 == 0 else t.clone()), D
     ld, ok = None, t.stride(-1) == 1 or D == 1
     for i in range(n - 2, -1, -1):                              # one stride for all rows together
         if t.shape[i] == 1:
@@ -189,26 +204,26 @@ def _rows(t):
 
 def _norm_operands(name, x, f, gate, residual_scale, w_post, w_pre):
     dt = _storage(name, x)
-    _need(x.dim() >= 1 and x.shape[-1] % 8 == 0 and 8 <= x.shape[-1] <= 8192, f'{name}: the width must be a multiple of 8 in [8, 8192]')
-    D = x.shape[-1]
+    D = x.shape[-1] if x.dim() else 0
+    _need(D % 8 == 0 and 8 <= D <= 8192, '{}: the width must be a multiple of 8 in [8, 8192]', name)
     rows = x.numel() // D
-    _need(f is not None or (gate is None and residual_scale is None and w_post is None),
-          f'{name}: gate, residual_scale and w_post belong to the block output f')
-    per = 0
     if f is not None:
         _like(name, 'f', f, x, x.shape)
+    elif gate is not None or residual_scale is not None or w_post is not None:
+        raise ValueError(f'{name}: gate, residual_scale and w_post belong to the block output f')
+    per = 0
     if gate is not None:
-        _need(gate.dtype == x.dtype and gate.device == x.device and gate.shape[-1] == D,
-              f'{name}: gate must have the width, dtype and device of x')
-        n = gate.numel() // D
-        # the gate's leading dimensions are x's up to some point, then ones: row r belongs to gate row r // per
-        lead, full = list(gate.shape[:-1]), list(x.shape[:-1])
-        _need(len(lead) <= len(full), f'{name}: gate has more dimensions than x')
-        lead += [1] * (len(full) - len(lead))
-        cut = max([i + 1 for i, s in enumerate(lead) if s != 1], default=0)
-        _need(lead[:cut] == full[:cut], f'{name}: gate {tuple(gate.shape)} must share the leading dimensions of x {tuple(x.shape)} '
-              'up to some point and have size 1 behind it')
-        per = rows // n if n else 1
+        per = 1
+        if gate.shape != x.shape:
+            # the gate's leading dimensions are x's up to some point, then ones: row r belongs to gate row r // per
+            lead, full = list(gate.shape[:-1]), list(x.shape[:-1])
+            cut = max([i + 1 for i, s in enumerate(lead) if s != 1], default=0)
+            _need(gate.dim() and gate.shape[-1] == D and len(lead) <= len(full) and lead[:cut] == full[:cut],
+                  '{}: gate {} must share the leading dimensions of x {} up to some point and have size 1 behind it',
+                  name, tuple(gate.shape), tuple(x.shape))
+            n = gate.numel() // D
+            per = rows // n if n else 1
+        _like(name, 'gate', gate, x, gate.shape)
     for what, w in (('residual_scale', residual_scale), ('w_post', w_post), ('w_pre', w_pre)):
         if w is not None:
             _like(name, what, w, x, (D,), torch.float32)
@@ -225,10 +240,10 @@ def norm_gate_fwd(x, f=None, gate=None, residual_scale=None, w_post=None, w_pre=
     name = 'norm_gate'
     dt, D, rows, per = _norm_operands(name, x, f, gate, residual_scale, w_post, w_pre)
     want_y = want_y and f is not None
-    _need(want_y or want_h, f'{name}: one of y, h must be wanted')
-    _need(want_h or w_pre is None, f'{name}: w_pre belongs to h')
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_y else None
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_h else None
+    _need(want_y or want_h, '{}: one of y, h must be wanted', name)
+    _need(want_h or w_pre is None, '{}: w_pre belongs to h', name)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format) if want_y else None
+    h = torch.empty_like(x, memory_format=torch.contiguous_format) if want_h else None
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if save else None
     if rows == 0:
         return y, h, stats
@@ -244,8 +259,8 @@ def norm_gate_bwd(dy, dh, x, stats, f=None, gate=None, residual_scale=None, w_po
     dw_pre), None for what was not given (dgate in the gate's shape, summed over the rows that share a gate row)."""
     name = 'norm_gate'
     dt, D, rows, per = _norm_operands(name, x, f, gate, residual_scale, w_post, w_pre)
-    _need(dy is not None or dh is not None, f'{name}: one of dy, dh is needed')
-    _need(dy is None or f is not None, f'{name}: without f there is no y, so no dy')
+    _need(dy is not None or dh is not None, '{}: one of dy, dh is needed', name)
+    _need(dy is None or f is not None, '{}: without f there is no y, so no dy', name)
     for what, g in (('dy', dy), ('dh', dh)):
         if g is not None:
             _like(name, what, g, x, x.shape)
@@ -263,7 +278,7 @@ def norm_gate_bwd(dy, dh, x, stats, f=None, gate=None, residual_scale=None, w_po
         return dx, df, dgate, drho, dw_post, dw_pre
     (x, ldx), (f, ldf), (gate, ldg), (dy, lddy), (dh, lddh) = _rows(x), _rows(f), _rows(gate), _rows(dy), _rows(dh)
     rho, w_post, w_pre, stats = _packed(residual_scale), _packed(w_post), _packed(w_pre), _packed(stats)
-    ws = _workspace(_lib.call('vqa_norm_gate_workspace_floats', rows, D, per), x.device)
+    ws = _workspace(_entry('vqa_norm_gate_workspace_floats')(rows, D, per), x.device)
     _call(x.device, 'vqa_norm_gate_bwd', _ptr(dy), lddy, _ptr(dh), lddh, x.data_ptr(), ldx, _ptr(f), ldf, _ptr(gate), ldg, per,
           _ptr(rho), _ptr(w_post), _ptr(w_pre), stats.data_ptr(), dx.data_ptr(), D, _ptr(df), D, _ptr(dgate), D,
           _ptr(drho), _ptr(dw_post), _ptr(dw_pre), ws.data_ptr(), rows, D, dt)
@@ -296,28 +311,30 @@ def norm_gate(x, f=None, gate=None, residual_scale=None, w_post=None, w_pre=None
 
 def _view(t):
     """(tensor, VqaAttnView) of a (B, T, H, D) operand, copied if the kernels cannot read its strides."""
-    st = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
-    if (t.stride(3) != 1 and t.shape[3] != 1) or any(s % 8 or s < 0 for s in st[:3]) or t.data_ptr() % 16:
+    sb, st, sh, one = t.stride()
+    nb, nt, nh, D = t.shape                                      # the stride of a size of 1 says nothing
+    sb, st, sh = sb if nb > 1 else 0, st if nt > 1 else 0, sh if nh > 1 else 0
+    if one != 1 or (sb | st | sh) % 8 or sb < 0 or st < 0 or sh < 0 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        st = t.stride()
-    return t, _lib.AttnView(t.data_ptr(), st[0], st[1], st[2])
+        sb, st, sh, one = t.stride()
+    return t, _lib.AttnView(t.data_ptr(), sb, st, sh)
 
 
 def _attn_operands(q, k, v, kv_len, mask, scale):
     name = 'cross_attention'
     dt = _storage(name, q)
-    _need(q.dim() == 4 and k.dim() == 4, f'{name}: q is (B, Tq, H, D), k and v are (B, Tk, Hkv, D)')
+    _need(q.dim() == 4 and k.dim() == 4, '{}: q is (B, Tq, H, D), k and v are (B, Tk, Hkv, D)', name)
     B, Tq, H, D = q.shape
-    Tk, Hkv = k.shape[1], k.shape[2]
+    _, Tk, Hkv, _ = k.shape
     _like(name, 'k', k, q, (B, Tk, Hkv, D))
     _like(name, 'v', v, q, (B, Tk, Hkv, D))
-    _need(Hkv > 0 and H > 0 and H % Hkv == 0, f'{name}: {H} query heads cannot share {Hkv} key heads evenly')
-    _need(D % 8 == 0 and 8 <= D <= 128, f'{name}: the head width must be a multiple of 8 in [8, 128], got {D}')
+    _need(Hkv > 0 and H > 0 and H % Hkv == 0, '{}: {} query heads cannot share {} key heads evenly', name, H, Hkv)
+    _need(D % 8 == 0 and 8 <= D <= 128, '{}: the head width must be a multiple of 8 in [8, 128], got {}', name, D)
     mask_sb = 0
     if mask is not None:
-        _need(tuple(mask.shape) == (B, Tk) and mask.device == q.device and mask.dtype in (torch.bool, torch.uint8),
-              f'{name}: mask must be ({B}, {Tk}) bool or uint8 on {q.device}')
-        if (Tk > 1 and mask.stride(1) != 1) or mask.stride(0) < 0:
+        _need(mask.shape == (B, Tk) and mask.device == q.device and mask.dtype in (torch.bool, torch.uint8),
+              '{}: mask must be ({}, {}) bool or uint8 on {}', name, B, Tk, q.device)
+        if Tk > 1 and mask.stride(1) != 1:
             mask = mask.contiguous()
         mask_sb = mask.stride(0)
     return dt, _lengths(name, 'kv_len', kv_len, q, B), mask, mask_sb, D ** -0.5 if scale is None else float(scale), B, Tq, Tk, H, Hkv, D
@@ -337,7 +354,7 @@ def cross_attention_fwd(q, k, v, kv_len=None, mask=None, scale=None):
     if B == 0 or Tq == 0 or Tk == 0:
         return o.zero_(), lse.fill_(float('-inf'))
     (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
-    ws = _workspace(_lib.call('vqa_cross_attn_fwd_workspace_floats', B, Tq, Tk, H, Hkv, D, dt), dev)
+    ws = _workspace(_entry('vqa_cross_attn_fwd_workspace_floats')(B, Tq, Tk, H, Hkv, D, dt), dev)
     _call(dev, 'vqa_cross_attn_fwd', byref(vq), byref(vk), byref(vv), _ptr(kv_len), _ptr(mask), mask_sb, scale, o.data_ptr(),
           lse.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
     return o, lse
@@ -356,7 +373,7 @@ def cross_attention_bwd(do, q, k, v, o, lse, kv_len=None, mask=None, scale=None)
         return dq.zero_(), dk.zero_(), dv.zero_()
     (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
     do, o, lse = _packed(do), _packed(o), _packed(lse)
-    ws = _workspace(_lib.call('vqa_cross_attn_bwd_workspace_floats', B, Tq, Tk, H, Hkv, D, dt), dev)
+    ws = _workspace(_entry('vqa_cross_attn_bwd_workspace_floats')(B, Tq, Tk, H, Hkv, D, dt), dev)
     _call(dev, 'vqa_cross_attn_bwd', do.data_ptr(), byref(vq), byref(vk), byref(vv), o.data_ptr(), lse.data_ptr(), _ptr(kv_len),
           _ptr(mask), mask_sb, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
     return dq, dk, dv
