@@ -443,26 +443,28 @@ int vqa_gated_scan_bwd(const void* dh, const float* dc_last, const void* gates, 
 /* Cross attention of Tq token rows to Tk region rows, H query heads on Hkv key heads (head h reads key head h / (H / Hkv)):
  *   o[b,t,h] = sum_r p_r v[b,r],  p = softmax_r(scale * q[b,t,h].k[b,r])  over the regions r < kv_len[b] with mask[b,r] != 0
  *   q (B, Tq, H, D), k and v (B, Tk, Hkv, D) are views: row (b, t, h) at data + b * sb + t * st + h * sh (elements,
- *               multiples of 8), D contiguous
- *   kv_len      optional (B), clamped to [0, Tk]; mask optional bytes, row b at mask + b * mask_sb.  Rows of k and v that
- *               do not count are not read, and their gradients are 0
+ *               multiples of 8, st < 2^26), D contiguous
+ *   kv_len      optional (B), clamped to [0, Tk]; mask optional bytes, row b at mask + b * mask_sb.  What rows of k and v
+ *               that do not count hold, NaN included, has no effect, and their gradients are 0
  *   o           (B, Tq, H, D) contiguous; a row with no region that counts is 0
+ *   o_rest      bf16 storage only, as o: what rounding took from o, for the backward (its sums of dO o are subtracted from
+ *               dO v, and with few regions, or one that has most of the weight, little is left of either); may be NULL
  *   lse         (B, H, Tq) fp32 log-sum-exp of a row's scores (-inf for such a row), for the backward; may be NULL
  *   workspace   vqa_cross_attn_{fwd,bwd}_workspace_floats fp32 (may be 0: NULL), scratch of one call
  * One query row against many regions (serving) is Tq = 1: the H / Hkv heads of a key head share one reading of it, and the
  * regions are split over workgroups where the batch does not fill the chip.
  * Backward: d_o as o; dq as o, dk and dv (B, Tk, Hkv, D) contiguous, summed over the heads that share a key head.
  * Scores, softmax and sums are fp32; with bf16 storage p and its gradient are rounded to bf16 for the products.
- * D % 8 == 0, D <= VQA_CROSS_ATTN_MAX_D, B * Tq * H <= 2^27, Tk <= 2^24. */
+ * D % 8 == 0, D <= VQA_CROSS_ATTN_MAX_D, B * Tq * H <= 2^27, Tk <= 2^24, Hkv * D < 2^26. */
 #define VQA_CROSS_ATTN_MAX_D 128
 typedef struct VqaAttnView { const void* data; long sb, st, sh; } VqaAttnView;
 size_t vqa_cross_attn_fwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype);
 size_t vqa_cross_attn_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype);
 int vqa_cross_attn_fwd(const VqaAttnView* q, const VqaAttnView* k, const VqaAttnView* v, const int32_t* kv_len,
-                       const uint8_t* mask, long mask_sb, float scale, void* o, float* lse, float* workspace, int B, int Tq,
-                       int Tk, int H, int Hkv, int D, int dtype, hipStream_t stream);
+                       const uint8_t* mask, long mask_sb, float scale, void* o, void* o_rest, float* lse, float* workspace, int B,
+                       int Tq, int Tk, int H, int Hkv, int D, int dtype, hipStream_t stream);
 int vqa_cross_attn_bwd(const void* d_o, const VqaAttnView* q, const VqaAttnView* k, const VqaAttnView* v, const void* o,
-                       const float* lse, const int32_t* kv_len, const uint8_t* mask, long mask_sb, float scale, void* dq,
+                       const void* o_rest, const float* lse, const int32_t* kv_len, const uint8_t* mask, long mask_sb, float scale, void* dq,
                        void* dk, void* dv, float* workspace, int B, int Tq, int Tk, int H, int Hkv, int D, int dtype,
                        hipStream_t stream);
 

@@ -57,9 +57,9 @@ def _bounds(q, k, v, do, o, lse, live, scale):
 
 def _run(q, k, v, do, kv_len=None, mask=None, scale=None):
     from vqa_amd import ops
-    o, lse = ops.cross_attention_fwd(q, k, v, kv_len, mask, scale)
-    grads = ops.cross_attention_bwd(do, q, k, v, o, lse, kv_len, mask, scale)
-    return (o, lse, *grads)
+    o, saved = ops.cross_attention_fwd(q, k, v, kv_len, mask, scale)
+    grads = ops.cross_attention_bwd(do, q, k, v, o, saved, kv_len, mask, scale)
+    return (o, saved[0], *grads)
 
 
 def _check(q, k, v, do, kv_len=None, mask=None, scale=None):
@@ -185,7 +185,8 @@ def test_empty_sizes():
     from vqa_amd import ops
     for B, Tq, Tk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
         q, k = torch.randn(B, Tq, 2, 8, device='cuda'), torch.randn(B, Tk, 1, 8, device='cuda')
-        o, lse = ops.cross_attention_fwd(q, k, k)
-        assert o.shape == q.shape and float(o.abs().sum()) == 0 and lse.shape == (B, 2, Tq)
-        dq, dk, dv = ops.cross_attention_bwd(o, q, k, k, o, lse)
+        o, saved = ops.cross_attention_fwd(q, k, k)
+        assert o.shape == q.shape and float(o.abs().sum()) == 0 and saved[0].shape == (B, 2, Tq)
+        assert ops.cross_attention_fwd(q, k, k, save=False)[1] is None
+        dq, dk, dv = ops.cross_attention_bwd(o, q, k, k, o, saved)
         assert dq.shape == q.shape and dk.shape == k.shape and float(dq.abs().sum() + dk.abs().sum() + dv.abs().sum()) == 0

@@ -89,8 +89,8 @@ _SIGNATURES = {
     'vqa_gated_scan_bwd': [_p, _p, _p, _l, _l, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     'vqa_cross_attn_fwd_workspace_floats': [_i, _i, _i, _i, _i, _i, _i],
     'vqa_cross_attn_bwd_workspace_floats': [_i, _i, _i, _i, _i, _i, _i],
-    'vqa_cross_attn_fwd': [_p, _p, _p, _p, _p, _l, _f, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
-    'vqa_cross_attn_bwd': [_p, _p, _p, _p, _p, _p, _p, _p, _l, _f, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
+    'vqa_cross_attn_fwd': [_p, _p, _p, _p, _p, _l, _f, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
+    'vqa_cross_attn_bwd': [_p, _p, _p, _p, _p, _p, _p, _p, _p, _l, _f, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p],
     'vqa_norm_gate_fwd': [_p, _l, _p, _l, _p, _l, _l, _p, _p, _p, _f, _p, _l, _p, _l, _p, _l, _i, _i, _p],
     'vqa_norm_gate_workspace_floats': [_l, _i, _l],
     'vqa_norm_gate_bwd': [_p, _l, _p, _l, _p, _l, _p, _l, _p, _l, _l, _p, _p, _p, _p, _p, _l, _p, _l, _p, _l, _p, _p, _p, _p, _l, _i, _i, _p],

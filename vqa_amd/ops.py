@@ -314,7 +314,7 @@ def _view(t):
     sb, st, sh, one = t.stride()
     nb, nt, nh, D = t.shape                                      # the stride of a size of 1 says nothing
     sb, st, sh = sb if nb > 1 else 0, st if nt > 1 else 0, sh if nh > 1 else 0
-    if one != 1 or (sb | st | sh) % 8 or sb < 0 or st < 0 or sh < 0 or t.data_ptr() % 16:
+    if one != 1 or (sb | st | sh) % 8 or sb < 0 or st < 0 or sh < 0 or st >= 1 << 26 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
         sb, st, sh, one = t.stride()
     return t, _lib.AttnView(t.data_ptr(), sb, st, sh)
@@ -340,58 +340,64 @@ def _attn_operands(q, k, v, kv_len, mask, scale):
     return dt, _lengths(name, 'kv_len', kv_len, q, B), mask, mask_sb, D ** -0.5 if scale is None else float(scale), B, Tq, Tk, H, Hkv, D
 
 
-def cross_attention_fwd(q, k, v, kv_len=None, mask=None, scale=None):
+def cross_attention_fwd(q, k, v, kv_len=None, mask=None, scale=None, save=True):
     """softmax(scale q k^T) v of the token rows ``q`` (B, Tq, H, D) over the regions ``k``, ``v`` (B, Tk, Hkv, D); head h
     reads key head h // (H // Hkv).
 
-    ``kv_len`` (B,): regions of each sample; ``mask`` (B, Tk): regions that count (True); what does not count is not
-    read.  ``scale`` defaults to D ** -0.5.  Returns o (B, Tq, H, D) and the log-sum-exp (B, H, Tq) float32 that
-    ``cross_attention_bwd`` needs; a row with nothing to attend gives 0 and -inf."""
+    ``kv_len`` (B,): regions of each sample; ``mask`` (B, Tk): regions that count (True); what does not count
+    may hold anything.  ``scale`` defaults to D ** -0.5.  Returns o (B, Tq, H, D), a row with nothing to attend 0, and what
+    ``cross_attention_bwd`` needs (None unless ``save``): the log-sum-exp of the scores (B, H, Tq) float32, -inf for such a
+    row, and for bfloat16 what rounding took from o."""
     dt, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D = _attn_operands(q, k, v, kv_len, mask, scale)
     dev = q.device
     o = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev)
+    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev) if save else None
+    rest = torch.empty_like(o) if save and dt == _lib.BF16 else None
     if B == 0 or Tq == 0 or Tk == 0:
-        return o.zero_(), lse.fill_(float('-inf'))
+        return o.zero_(), (lse.fill_(float('-inf')), rest if rest is None else rest.zero_()) if save else None
     (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
     ws = _workspace(_entry('vqa_cross_attn_fwd_workspace_floats')(B, Tq, Tk, H, Hkv, D, dt), dev)
     _call(dev, 'vqa_cross_attn_fwd', byref(vq), byref(vk), byref(vv), _ptr(kv_len), _ptr(mask), mask_sb, scale, o.data_ptr(),
-          lse.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
-    return o, lse
+          _ptr(rest), _ptr(lse), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
+    return o, (lse, rest) if save else None
 
 
-def cross_attention_bwd(do, q, k, v, o, lse, kv_len=None, mask=None, scale=None):
-    """Gradients (dq, dk, dv) of ``cross_attention_fwd`` from do (B, Tq, H, D) and what it returned."""
+def cross_attention_bwd(do, q, k, v, o, saved, kv_len=None, mask=None, scale=None):
+    """Gradients (dq, dk, dv) of ``cross_attention_fwd`` from do (B, Tq, H, D) and the two things it returned."""
     dt, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D = _attn_operands(q, k, v, kv_len, mask, scale)
     dev = q.device
     _like('cross_attention', 'do', do, q, q.shape)
     _like('cross_attention', 'o', o, q, q.shape)
-    _like('cross_attention', 'lse', lse, q, (B, H, Tq), torch.float32)
+    _need(saved is not None, 'cross_attention: the backward needs what cross_attention_fwd(..., save=True) returned')
+    lse, rest = saved
+    _like('cross_attention', 'the saved log-sum-exp', lse, q, (B, H, Tq), torch.float32)
+    if rest is not None:
+        _like('cross_attention', "the saved rest of o", rest, q, q.shape)
     dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
     dk, dv = (torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=dev) for _ in range(2))
     if B == 0 or Tq == 0 or Tk == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
-    do, o, lse = _packed(do), _packed(o), _packed(lse)
+    do, o, lse, rest = _packed(do), _packed(o), _packed(lse), _packed(rest)
     ws = _workspace(_entry('vqa_cross_attn_bwd_workspace_floats')(B, Tq, Tk, H, Hkv, D, dt), dev)
-    _call(dev, 'vqa_cross_attn_bwd', do.data_ptr(), byref(vq), byref(vk), byref(vv), o.data_ptr(), lse.data_ptr(), _ptr(kv_len),
-          _ptr(mask), mask_sb, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
+    _call(dev, 'vqa_cross_attn_bwd', do.data_ptr(), byref(vq), byref(vk), byref(vv), o.data_ptr(), _ptr(rest), lse.data_ptr(),
+          _ptr(kv_len), _ptr(mask), mask_sb, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
     return dq, dk, dv
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, kv_len, mask, scale):
-        o, lse = cross_attention_fwd(q, k, v, kv_len, mask, scale)
-        ctx.save_for_backward(q, k, v, o, lse, kv_len, mask)
+        o, saved = cross_attention_fwd(q, k, v, kv_len, mask, scale, save=any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, o, *(saved or (None, None)), kv_len, mask)
         ctx.scale = scale
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, kv_len, mask = ctx.saved_tensors
-        return (*cross_attention_bwd(do, q, k, v, o, lse, kv_len, mask, ctx.scale), None, None, None)
+        q, k, v, o, lse, rest, kv_len, mask = ctx.saved_tensors
+        return (*cross_attention_bwd(do, q, k, v, o, (lse, rest), kv_len, mask, ctx.scale), None, None, None)
 
 
 def cross_attention(q, k, v, kv_len=None, mask=None, scale=None):
