@@ -29,7 +29,7 @@ template <> struct Ty<bf16_t> {
     typedef s16x4_t half;                        // half of one: four values per lane
     static constexpr bool PARTS = true;          // a fp32 factor can be given in two parts
     static constexpr int E = 8, KC = 32, NS = 2; // elements per lane, contraction length, 16-row tiles per fragment's worth of rows
-    static constexpr int PAD = 32;               // LDS pitch = row bytes + PAD: rows fall on different banks for both kinds of reads
+    static constexpr int PAD = 16;               // LDS pitch = row bytes + PAD: rows fall on different banks for both kinds of reads
     static __device__ __forceinline__ f32x4 mma(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     // four fp32 values rounded to storage
     static __device__ __forceinline__ half pack(f32x4 v) {
@@ -42,10 +42,10 @@ template <> struct Ty<bf16_t> {
         for (int i = 0; i < 4; ++i) v[i] -= bf16_to_f32((bf16_t)h[i]);
         return pack(v);
     }
-    // product over 16 (contraction) with the second factor in its two parts: [a a] [hi lo]^T in one instruction
+    // product over 16 (contraction), the second factor in its two parts
     static __device__ __forceinline__ f32x4 mma_parts(half a, half hi, half lo, f32x4 c) {
-        const half aa[2] = {a, a}, bb[2] = {hi, lo};
-        return mma(join(aa), join(bb), c);
+        c = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, lo, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, hi, c, 0, 0, 0);
     }
     static __device__ __forceinline__ frag join(const half (&h)[2]) {
         const s16x8 v = {h[0][0], h[0][1], h[0][2], h[0][3], h[1][0], h[1][1], h[1][2], h[1][3]};
@@ -239,9 +239,14 @@ template <typename T, int DF> struct KeyTile {
     static __device__ __forceinline__ void put(const u32x4 (&r)[NI], const Spots<T, NI>& sp, const KeyBits<T>& bits, char* lds, int pitch) {
         const unsigned on = bits.b[0] | bits.b[Y::NS - 1] << (16 * (Y::NS - 1));
         const u32x4 z = {};
+        if (on == (Y::NS == 2 ? 0xffffffffu : 0xffffu)) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            *reinterpret_cast<u32x4*>(lds + sp.row(i) * pitch + sp.col(i) * (int)sizeof(T)) = (on >> sp.row(i)) & 1 ? r[i] : z;
+            for (int i = 0; i < NI; ++i) *reinterpret_cast<u32x4*>(lds + sp.row(i) * pitch + sp.col(i) * (int)sizeof(T)) = r[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                *reinterpret_cast<u32x4*>(lds + sp.row(i) * pitch + sp.col(i) * (int)sizeof(T)) = (on >> sp.row(i)) & 1 ? r[i] : z;
+        }
     }
 };
 // a wave's part of LDS cleared: the columns between D and the fragments' width stay zero from then on
@@ -337,6 +342,7 @@ __global__ void __launch_bounds__(256) k_xattn_fwd(Args<T> a) {
         for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float scale2 = a.scale * LOG2E;
+    const bool spare = a.D <= DP - 16;                       // the last 16 columns are all padding
     if (a.D < DP) wave_clear(my, TILE, lane);
 
     for (int tile = first + w0; tile < last; tile += W) {
@@ -397,6 +403,7 @@ __global__ void __launch_bounds__(256) k_xattn_fwd(Args<T> a) {
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
+            if (d == DT - 1 && spare) break;
             const frag vt = frag_t<T>(my, PITCH, d * 16, li, g);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -500,22 +507,25 @@ __global__ void __launch_bounds__(256) k_xattn_delta(Args<T> a, float* delta) {
     }
 }
 
-// Rows of a pair all on the chip (M <= 16 MT): ONE pass over the keys for all three gradients.  Per 16 keys: S (rows x
-// keys) and dP = dO V^T as result tiles, P and dS = P (dP - delta) from them; those are the B operands of dV^T = dO^T P and
-// dK^T = Q^T dS, whose tiles are complete and leave at once, by way of the values' rows of LDS so that whole rows are
-// written; dS^T, through 16 x 16 of LDS, is the B operand of dQ^T += K^T dS^T, which stays in registers and is joined over
-// waves (and key ranges) at the end.  P and dS enter their products in two bf16 parts: the work is bound by reading the keys
-// and writing their gradients, and only 16 of a matrix instruction's 32 contraction steps would be used otherwise.
+// Rows of a pair all on the chip (M <= 16 MT): ONE pass over the keys for all three gradients.  A tile's values pass
+// through the wave's LDS for dP = dO V^T, then its keys for S = Q K^T (result tiles of 16 rows x 16 keys); P and
+// dS = scale P (dP - delta) from them are the B operands of dV^T = dO^T P and dK^T = Q^T dS; dS^T, through 16 x 16 pieces of
+// LDS, is the B operand of dQ^T += K^T dS^T, which stays in registers and is joined over waves (and key ranges) at the
+// end.  dV and dK leave through the same LDS once the keys are done with, so that whole rows are written.  P and dS enter
+// their products in two bf16 parts: the work is bound by reading the keys and writing their gradients, and only 16 of a
+// matrix instruction's 32 contraction steps would be used otherwise.  Q^T and dO^T of up to 16 bf16 rows are held in
+// registers (HELD); others are read, transposed, from LDS, one copy per item.
 template <typename T, int DF, int MT, int W>
 __global__ void __launch_bounds__(256) k_xattn_bwd(Args<T> a) {
     typedef Ty<T> Y;
     typedef typename Y::frag frag;
     typedef typename Y::half half;
+    constexpr bool HELD = MT == 1 && Y::PARTS;
     constexpr int DP = DF * Y::KC, DT = DP / 16, PITCH = DP * (int)sizeof(T) + Y::PAD, OP = DP + 4;
-    constexpr int TILE = Y::KC * PITCH, JOIN = 4 * 16 * OP * 4, ROWS = MT * 16 * PITCH;
-    constexpr int SP = sizeof(T) == 4 ? 80 : 40, DS = 16 * SP;         // dS^T: keys x 16 rows
-    __shared__ __attribute__((aligned(16))) char lds[8 * TILE > JOIN ? 8 * TILE : JOIN];
-    __shared__ __attribute__((aligned(16))) char rows_lds[(4 / W) * 2 * ROWS], lds_ds[4 * DS];
+    constexpr int TILE = Y::KC * PITCH, JOIN = 4 * 16 * OP * 4, ROWS = HELD ? 0 : MT * 16 * PITCH;
+    constexpr int PIECES = Y::NS * (Y::PARTS ? 2 : 1), SP = sizeof(T) == 4 ? 80 : 40, DS = PIECES * 16 * SP;     // dS^T: keys x 16 rows
+    __shared__ __attribute__((aligned(16))) char lds[4 * TILE > JOIN ? 4 * TILE : JOIN];
+    __shared__ __attribute__((aligned(16))) char lds_ds[4 * DS], rows_lds[HELD ? 16 : (4 / W) * 2 * ROWS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, w0 = wave % W;
     const int wi_ = work_item(a.blocks) * (4 / W) + wave / W;
     const bool idle = wi_ >= a.items;                        // an item past the last one: no keys, nothing stored
@@ -526,10 +536,11 @@ __global__ void __launch_bounds__(256) k_xattn_bwd(Args<T> a) {
     const T* kb = a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh;
     const T* vb = a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh;
     const int first = split * a.tiles_split, last = idle ? 0 : min(first + a.tiles_split, (a.Tk + Y::KC - 1) / Y::KC);
-    char *lk = lds + wave * 2 * TILE, *lv = lk + TILE, *my_ds = lds_ds + wave * DS;
+    char *my = lds + wave * TILE, *my_ds = lds_ds + wave * DS;
     char *lq = rows_lds + (wave / W) * 2 * ROWS, *ldo = lq + ROWS;
     const float scale2 = a.scale * LOG2E;
     const unsigned out_st = a.Hkv * a.D;
+    const bool spare = a.D <= DP - 16;                       // the last 16 columns are all padding
 
     // everything that the first tile waits for is requested at once: rows, outputs, statistics, then the tile itself
     frag q[MT][DF], d_o[MT][DF], o[MT][DF], rest[MT][DF];
@@ -549,10 +560,8 @@ __global__ void __launch_bounds__(256) k_xattn_bwd(Args<T> a) {
     sp.init(lane, a.D, Y::KC);
     KeyTile<T, DF> nxt;
     nxt.load(a, sp, mask, len, kb, vb, (first + w0) * Y::KC, li);
-    if (a.D < DP) wave_clear(lk, 2 * TILE, lane);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const int m = mt * 16 + li;
         float s = 0.f, s_rest = 0.f;
 #pragma unroll
         for (int f = 0; f < DF; ++f) {
@@ -560,117 +569,140 @@ __global__ void __launch_bounds__(256) k_xattn_bwd(Args<T> a) {
             if constexpr (Y::PARTS) s_rest += Y::dot(d_o[mt][f], rest[mt][f]);
         }
         s = groups_sum(a.rest ? s + s_rest : s);
-        const float l = m < M ? row_lse[mt] * LOG2E : INFINITY;
+        const float l = mt * 16 + li < M ? row_lse[mt] * LOG2E : INFINITY;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             delta[mt][r] = __shfl(s, g * 4 + r, 64);
             lse[mt][r] = __shfl(l, g * 4 + r, 64);
         }
-        if (w0 == 0) {
-#pragma unroll
-            for (int f = 0; f < DF; ++f) {
-                *reinterpret_cast<frag*>(lq + m * PITCH + f * 64 + g * 16) = q[mt][f];
-                *reinterpret_cast<frag*>(ldo + m * PITCH + f * 64 + g * 16) = d_o[mt][f];
-            }
-        }
     }
+    half q_t[HELD ? DT : 1], do_t[HELD ? DT : 1];
+    auto rows_to = [&](char* to, const frag (&r)[MT][DF]) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int f = 0; f < DF; ++f) *reinterpret_cast<frag*>(to + (mt * 16 + li) * PITCH + f * 64 + g * 16) = r[mt][f];
+    };
+    if constexpr (HELD) {
+        rows_to(my, q);
+        wave_lds_order();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) q_t[d] = Y::read_t(my, PITCH, g * 4, d * 16, li);
+        wave_lds_order();
+        rows_to(my, d_o);
+        wave_lds_order();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) do_t[d] = Y::read_t(my, PITCH, g * 4, d * 16, li);
+        wave_lds_order();
+    } else {
+        if (w0 == 0) { rows_to(lq, q); rows_to(ldo, d_o); }
+        __syncthreads();
+    }
+    if (a.D < DP) wave_clear(my, TILE, lane);
     f32x4 dq[MT][DT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int d = 0; d < DT; ++d) dq[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    __syncthreads();
 
     for (int tile = first + w0; tile < last; tile += W) {
         const int key0 = tile * Y::KC;
+        const KeyBits<T> bits = nxt.bits(mask != nullptr, len, key0, li);
         wave_lds_order();
-        const KeyBits<T> bits = nxt.bits(mask != nullptr, len, tile * Y::KC, li);
-        nxt.put(nxt.k, sp, bits, lk, PITCH);
-        nxt.put(nxt.v, sp, bits, lv, PITCH);
+        nxt.put(nxt.v, sp, bits, my, PITCH);
         wave_lds_order();
-        nxt.load(a, sp, mask, len, kb, vb, key0 + W * Y::KC, li);
-        half dst[MT][Y::NS], dst_lo[MT][Y::NS];
+        nxt.load_v(a, sp, len, vb, key0 + W * Y::KC);
+        f32x4 s[Y::NS][MT], dp[Y::NS][MT];
 #pragma unroll
         for (int ns = 0; ns < Y::NS; ++ns) {
-            half p[MT], p_lo[MT], ds[MT], ds_lo[MT];
-            f32x4 s[MT], dp[MT];
-            const bool on = (bits.b[ns] >> li) & 1;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) s[mt] = dp[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int mt = 0; mt < MT; ++mt) s[ns][mt] = dp[ns][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int f = 0; f < DF; ++f) {
-                const frag k = frag_at<T>(lk, PITCH, ns * 16 + li, f, g), v = frag_at<T>(lv, PITCH, ns * 16 + li, f, g);
+                const frag v = frag_at<T>(my, PITCH, ns * 16 + li, f, g);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    s[mt] = Y::mma(q[mt][f], k, s[mt]);
-                    dp[mt] = Y::mma(d_o[mt][f], v, dp[mt]);
-                }
+                for (int mt = 0; mt < MT; ++mt) dp[ns][mt] = Y::mma(d_o[mt][f], v, dp[ns][mt]);
             }
+        }
+        wave_lds_order();
+        nxt.put(nxt.k, sp, bits, my, PITCH);
+        wave_lds_order();
+        nxt.load_k(a, sp, mask, len, kb, key0 + W * Y::KC, li);
+        half p[Y::NS][MT], p_lo[Y::NS][MT], ds[Y::NS][MT], ds_lo[Y::NS][MT];
+#pragma unroll
+        for (int ns = 0; ns < Y::NS; ++ns) {
+#pragma unroll
+            for (int f = 0; f < DF; ++f) {
+                const frag k = frag_at<T>(my, PITCH, ns * 16 + li, f, g);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[ns][mt] = Y::mma(q[mt][f], k, s[ns][mt]);
+            }
+            const bool on = (bits.b[ns] >> li) & 1;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[mt][r] = on ? __builtin_amdgcn_exp2f(s[mt][r] * scale2 - lse[mt][r]) : 0.f;
-                    dp[mt][r] = on ? s[mt][r] * (dp[mt][r] - delta[mt][r]) : 0.f;
+                    s[ns][mt][r] = on ? __builtin_amdgcn_exp2f(s[ns][mt][r] * scale2 - lse[mt][r]) : 0.f;
+                    dp[ns][mt][r] = on ? s[ns][mt][r] * (dp[ns][mt][r] - delta[mt][r]) * a.scale : 0.f;
                 }
-                p[mt] = Y::pack(s[mt]);
-                ds[mt] = Y::pack(dp[mt]);
-                p_lo[mt] = Y::rest(s[mt], p[mt]);
-                ds_lo[mt] = Y::rest(dp[mt], ds[mt]);
+                p[ns][mt] = Y::pack(s[ns][mt]);
+                ds[ns][mt] = Y::pack(dp[ns][mt]);
+                p_lo[ns][mt] = Y::rest(s[ns][mt], p[ns][mt]);
+                ds_lo[ns][mt] = Y::rest(dp[ns][mt], ds[ns][mt]);
             }
-            char* out = lv + ns * 16 * PITCH;                // these 16 keys' values are done with
-            auto leave = [&](T* dst_) {
-                wave_lds_order();
-                const int k0 = key0 + ns * 16, n = max(min(16, a.Tk - k0), 0);
-                const Window w(dst_ + (((size_t)b * a.Tk + k0) * a.Hkv + hk) * a.D, n ? ((n - 1) * out_st + a.D) * (unsigned)sizeof(T) : 0);
+        }
+        half dst[MT][Y::NS], dst_lo[MT][Y::NS];
 #pragma unroll
-                for (int i = 0; i < DF; ++i)                 // (the first 16 rows' chunks lie in the first half)
-                    w.store(sp.row(i) < 16 ? sp.at(i, out_st) : 0xffffff00u,
-                            *reinterpret_cast<const u32x4*>(out + (sp.row(i) & 15) * PITCH + sp.col(i) * (int)sizeof(T)));
-                wave_lds_order();
-            };
+        for (int mt = 0; mt < MT; ++mt) {                    // dS^T by way of LDS: lane writes rows 4 g + r of key li
             wave_lds_order();
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                f32x4 dv = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                    dv = Y::mma_parts(Y::read_t(ldo, PITCH, mt * 16 + g * 4, d * 16, li), p[mt], p_lo[mt], dv);
-                store4(reinterpret_cast<T*>(out + li * PITCH) + d * 16 + g * 4, dv);
+            for (int ns = 0; ns < Y::NS; ++ns) {
+                *reinterpret_cast<half*>(my_ds + (ns * 16 + li) * SP + g * (int)sizeof(half)) = ds[ns][mt];
+                if constexpr (Y::PARTS) *reinterpret_cast<half*>(my_ds + ((Y::NS + ns) * 16 + li) * SP + g * (int)sizeof(half)) = ds_lo[ns][mt];
             }
-            leave(a.dv);
+            wave_lds_order();
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                f32x4 dk = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-                    dk = Y::mma_parts(Y::read_t(lq, PITCH, mt * 16 + g * 4, d * 16, li), ds[mt], ds_lo[mt], dk);
-                store4(reinterpret_cast<T*>(out + li * PITCH) + d * 16 + g * 4, dk * a.scale);
-            }
-            leave(a.dk);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {                // dS^T by way of LDS: lane writes rows 4 g + r of key li
-                wave_lds_order();
-                *reinterpret_cast<half*>(my_ds + li * SP + g * (int)sizeof(half)) = ds[mt];
-                wave_lds_order();
-                dst[mt][ns] = Y::read_t(my_ds, SP, g * 4, 0, li);
-                if constexpr (Y::PARTS) {
-                    wave_lds_order();
-                    *reinterpret_cast<half*>(my_ds + li * SP + g * (int)sizeof(half)) = ds_lo[mt];
-                    wave_lds_order();
-                    dst_lo[mt][ns] = Y::read_t(my_ds, SP, g * 4, 0, li);
-                }
+            for (int ns = 0; ns < Y::NS; ++ns) {
+                dst[mt][ns] = Y::read_t(my_ds, SP, ns * 16 + g * 4, 0, li);
+                if constexpr (Y::PARTS) dst_lo[mt][ns] = Y::read_t(my_ds, SP, (Y::NS + ns) * 16 + g * 4, 0, li);
             }
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            const frag kt = frag_t<T>(lk, PITCH, d * 16, li, g);
+            if (d == DT - 1 && spare) break;
+            const frag kt = frag_t<T>(my, PITCH, d * 16, li, g);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 dq[mt][d] = Y::mma(kt, Y::join(dst[mt]), dq[mt][d]);
                 if constexpr (Y::PARTS) dq[mt][d] = Y::mma(kt, Y::join(dst_lo[mt]), dq[mt][d]);
             }
         }
+        // the tile's gradients: result tiles to LDS (over the keys), rows to memory
+        auto leave = [&](T* to, const half (&held)[HELD ? DT : 1], const char* from, const half (&x)[Y::NS][MT], const half (&x_lo)[Y::NS][MT]) {
+            wave_lds_order();
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                if (d == DT - 1 && spare) break;
+#pragma unroll
+                for (int ns = 0; ns < Y::NS; ++ns) {
+                    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if constexpr (HELD) y = Y::mma_parts(held[d], x[ns][mt], x_lo[ns][mt], y);
+                        else y = Y::mma_parts(Y::read_t(from, PITCH, mt * 16 + g * 4, d * 16, li), x[ns][mt], x_lo[ns][mt], y);
+                    }
+                    store4(reinterpret_cast<T*>(my + (ns * 16 + li) * PITCH) + d * 16 + g * 4, y);
+                }
+            }
+            wave_lds_order();
+            const int n = min(Y::KC, a.Tk - key0);
+            const Window w(to + (((size_t)b * a.Tk + key0) * a.Hkv + hk) * a.D, ((n - 1) * out_st + a.D) * (unsigned)sizeof(T));
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+                w.store(sp.at(i, out_st), *reinterpret_cast<const u32x4*>(my + sp.row(i) * PITCH + sp.col(i) * (int)sizeof(T)));
+        };
+        leave(a.dv, do_t, ldo, p, p_lo);
+        leave(a.dk, q_t, lq, ds, ds_lo);
     }
 
     float* jo = reinterpret_cast<float*>(lds);
@@ -688,7 +720,7 @@ __global__ void __launch_bounds__(256) k_xattn_bwd(Args<T> a) {
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < W; ++i) x += *reinterpret_cast<const f32x4*>(jo + ((wave - w0 + i) * 16 + r) * OP + col);
-            if (a.nsplit == 1) store4(a.dq + row_at(a, b, hk, m) + col, x * a.scale);
+            if (a.nsplit == 1) store4(a.dq + row_at(a, b, hk, m) + col, x);
             else *reinterpret_cast<f32x4*>(a.ws + ((size_t)split * rows + (size_t)pair * a.M + m) * a.D + col) = x;
         }
     }
@@ -704,7 +736,7 @@ __global__ void __launch_bounds__(256) k_xattn_dq_join(Args<T> a) {
     const int col = (int)(id % chunks) * 4, pair = (int)(row / a.M), m = (int)(row % a.M);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < a.nsplit; ++s) v += *reinterpret_cast<const f32x4*>(a.ws + (s * rows + row) * a.D + col);
-    store4(a.dq + row_at(a, pair / a.Hkv, pair % a.Hkv, m) + col, v * a.scale);
+    store4(a.dq + row_at(a, pair / a.Hkv, pair % a.Hkv, m) + col, v);
 }
 
 // More rows than fit: the rows' side (dq) as the forward does it, rows in registers, key tiles streamed ...
