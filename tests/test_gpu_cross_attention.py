@@ -94,7 +94,10 @@ def _check(q, k, v, do, kv_len=None, mask=None, scale=None):
 SHAPES = [  # B, Tq, Tk, H, Hkv, D
     (1, 1, 1, 1, 1, 8), (2, 1, 15, 2, 1, 16), (1, 3, 16, 4, 4, 24), (3, 2, 17, 8, 2, 40), (2, 14, 33, 3, 3, 80),
     (2, 5, 196, 12, 4, 64), (1, 1, 700, 16, 2, 128), (2, 16, 63, 2, 2, 96), (2, 17, 65, 2, 2, 72), (1, 20, 129, 6, 3, 32),
-    (2, 33, 50, 4, 4, 56), (1, 65, 130, 8, 2, 112), (1, 130, 577, 2, 1, 128), (3, 40, 7, 4, 1, 48), (1, 8, 2000, 8, 1, 88)]
+    (2, 33, 50, 4, 4, 56), (1, 65, 130, 8, 2, 112), (1, 130, 577, 2, 1, 128), (3, 40, 7, 4, 1, 48), (1, 8, 2000, 8, 1, 88),
+    # more than 64 rows on more than 256 regions: the matrix-bound kernels, each width and both workgroup sizes
+    (1, 70, 300, 1, 1, 24), (2, 100, 513, 2, 2, 64), (1, 40, 260, 8, 2, 96), (1, 150, 321, 2, 1, 80), (1, 257, 700, 1, 1, 120),
+    (2, 33, 449, 6, 2, 104), (1, 20, 385, 16, 2, 8)]
 
 
 @pytest.mark.parametrize('B,Tq,Tk,H,Hkv,D', SHAPES)

@@ -493,10 +493,17 @@ __global__ void __launch_bounds__(256) k_xattn_delta(Args<T> a, float* delta) {
     const int li = threadIdx.x & 15;
     if (row >= rows) return;
     float s = 0.f;
-    for (int c = li * 4; c < a.D; c += 64) {
-        const T *p = a.dout + row * a.D + c, *q = a.o + row * a.D + c;
+    for (int c = li * 8; c < a.D; c += 128) {
+        float x[8], y[8], z[8];
+        Vec8<T>::load(a.dout + row * a.D + c, x);
+        Vec8<T>::load(a.o + row * a.D + c, y);
+        if (a.rest) {
+            Vec8<T>::load(a.rest + row * a.D + c, z);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s += to_f32(p[i]) * (to_f32(q[i]) + (a.rest ? to_f32(a.rest[row * a.D + c + i]) : 0.f));
+            for (int i = 0; i < 8; ++i) y[i] += z[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += x[i] * y[i];
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
@@ -961,35 +968,480 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_kv(Args<T> a) {
     }
 }
 
+// ---- many rows and many keys ------------------------------------------------------------------
+// Beyond 64 rows and 256 keys the matrix cores are the bound (14 M Tk / (M + Tk) flops per byte and 16-bit element, against
+// 230 that the card does per byte it reads), and what feeds them is LDS: a wave that reads a 16 x 16 key fragment once for
+// two row tiles keeps LDS as busy as the matrix core.  Keys (rows, in the keys' backward) lie in LDS, two tiles of 64, for
+// eight waves of 32 rows each; the next tile is in flight in registers.  P and dS are rounded to bf16 for their products
+// (2^-9 of every term at random, over more than 256 terms).
+
+// R rows (64 or 32) of two operands on their way to LDS, NW waves together
+template <int DF, int NW, int R = 64> struct RowTile {
+    static constexpr int DP = DF * 32, PITCH = DP * 2 + 16, TILE = R * PITCH, NI = (4 * DF * R + NW * 64 - 1) / (NW * 64);
+    u32x4 x[NI], y[NI];
+    int rc[NI];                                              // row | chunk << 8
+    __device__ __forceinline__ void init(int D) {
+        const unsigned per = D / 8, inv = (65536 + per - 1) / per;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const unsigned c = min((unsigned)(i * NW * 64 + threadIdx.x), per * R - 1), r = (c * inv) >> 16;
+            rc[i] = (int)(r | (c - r * per) << 8);
+        }
+    }
+    __device__ __forceinline__ unsigned row(int i) const { return rc[i] & 255; }
+    __device__ __forceinline__ unsigned col(int i) const { return (rc[i] >> 8) * 8; }
+    // rows of one stride (keys)
+    static __device__ __forceinline__ Window window(const bf16_t* base, long st, long row0, int rows, int D) {
+        return Window(base + (size_t)row0 * st, rows > 0 ? ((rows - 1) * (unsigned)st + D) * 2u : 0u);
+    }
+    __device__ __forceinline__ void put(char* lx, char* ly, unsigned long long on) const {
+        const u32x4 z = {};
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const bool here = (on >> row(i)) & 1;
+            const int at = row(i) * PITCH + col(i) * 2;
+            *reinterpret_cast<u32x4*>(lx + at) = here ? x[i] : z;
+            *reinterpret_cast<u32x4*>(ly + at) = here ? y[i] : z;
+        }
+    }
+};
+
+// which of 64 keys count, one bit per key; the mask's bytes are requested with the tile
+struct Live64 {
+    unsigned m;
+    __device__ __forceinline__ void load(const uint8_t* mask, const void* any, int key0, int Tk, int lane) {
+        const uint8_t* p = mask ? mask : reinterpret_cast<const uint8_t*>(any);
+        m = p[mask ? min(key0 + lane, Tk - 1) : 0];
+    }
+    __device__ __forceinline__ unsigned long long bits(bool masked, int len, int key0, int lane) const {
+        return __ballot(key0 + lane < len && (!masked || m != 0));
+    }
+};
+
+// the workgroup's LDS cleared (pad columns stay zero)
+__device__ __forceinline__ void group_clear(char* lds, int bytes) {
+    const f32x4 z = {};
+    for (int at = threadIdx.x * 16; at < bytes; at += blockDim.x * 16) *reinterpret_cast<f32x4*>(lds + at) = z;
+}
+
+template <int DF, int NW>
+__global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
+    typedef Ty<bf16_t> Y;
+    typedef RowTile<DF, NW> Tile;
+    constexpr int DT = DF * 2, PITCH = Tile::PITCH, MT = 2;
+    __shared__ __attribute__((aligned(16))) char lds[4 * Tile::TILE];
+    const int wi = work_item(a.blocks);
+    if (wi >= a.blocks) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int rb = wi % a.row_blocks, ps = wi / a.row_blocks, split = ps % a.nsplit, pair = ps / a.nsplit;
+    const int b = pair / a.Hkv, hk = pair % a.Hkv, m0 = (rb * NW + wave) * 16 * MT;
+    const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
+    const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
+    const bf16_t* kb = a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh;
+    const bf16_t* vb = a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh;
+    const int first = split * a.tiles_split, last = min(first + a.tiles_split, (len + 63) / 64);
+
+    bf16x8_t q[MT][DF];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+        load_rows<bf16_t, DF>(a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh, a.q_st, a.q_sh, m0 + mt * 16 + li, a.M, a.G, a.D, g, q[mt]);
+    Tile nxt;
+    Live64 live;
+    nxt.init(a.D);
+    auto load = [&](int tile) {
+        const int key0 = tile * 64, rows = min(64, len - key0);
+        live.load(mask, kb, key0, a.Tk, lane);
+        const Window kw = Tile::window(kb, a.k_st, key0, rows, a.D), vw = Tile::window(vb, a.v_st, key0, rows, a.D);
+#pragma unroll
+        for (int i = 0; i < Tile::NI; ++i) {
+            nxt.x[i] = kw.load((nxt.row(i) * (unsigned)a.k_st + nxt.col(i)) * 2u);
+            nxt.y[i] = vw.load((nxt.row(i) * (unsigned)a.v_st + nxt.col(i)) * 2u);
+        }
+    };
+    load(first);
+    f32x4 o[MT][DT];
+    float mx[MT], sum[MT];                                   // mx: in units of the unscaled score
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        mx[mt] = -INFINITY;
+        sum[mt] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float scale2 = a.scale * LOG2E;
+    if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
+    unsigned long long on = live.bits(mask != nullptr, len, first * 64, lane), on_next = 0;
+    nxt.put(lds, lds + Tile::TILE, on);
+    load(first + 1);
+    __syncthreads();
+
+    int cur = 0;
+    for (int tile = first; tile < last; ++tile) {
+        const char *lk = lds + cur * 2 * Tile::TILE, *lv = lk + Tile::TILE;
+        f32x4 s[MT][4];
+#pragma unroll
+        for (int sub = 0; sub < 4; ++sub) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) s[mt][sub] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int f = 0; f < DF; ++f) {
+                const bf16x8_t k = frag_at<bf16_t>(lk, PITCH, sub * 16 + li, f, g);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][sub] = Y::mma(k, q[mt][f], s[mt][sub]);
+            }
+        }
+        bf16x8_t p[MT][2];
+        const bool full = on == ~0ull;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[mt][sub][r] *= scale2;
+                    if (!full) s[mt][sub][r] = (on >> (sub * 16 + g * 4 + r)) & 1 ? s[mt][sub][r] : -INFINITY;
+                    top = fmaxf(top, s[mt][sub][r]);
+                }
+            top = groups_max(top);
+            // the maximum follows only when a row's has grown by more than 2^8: until then p stays below 256, which
+            // costs no accuracy, and the output need not be rescaled
+            if (__any(top > mx[mt] + 8.f)) {
+                const float up = fmaxf(top, mx[mt]), at = up == -INFINITY ? 0.f : up, shrink = __builtin_amdgcn_exp2f(mx[mt] - at);
+                mx[mt] = up;
+                sum[mt] *= shrink;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[mt][d] *= shrink;
+            }
+            const float at = mx[mt] == -INFINITY ? 0.f : mx[mt];
+            Y::half h[4];
+#pragma unroll
+            for (int sub = 0; sub < 4; ++sub) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[mt][sub][r] = __builtin_amdgcn_exp2f(s[mt][sub][r] - at);
+                    sum[mt] += s[mt][sub][r];
+                }
+                h[sub] = Y::pack(s[mt][sub]);
+            }
+            const Y::half h0[2] = {h[0], h[1]}, h1[2] = {h[2], h[3]};
+            p[mt][0] = Y::join(h0);
+            p[mt][1] = Y::join(h1);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const bf16x8_t vt = frag_t<bf16_t>(lv + kk * 32 * PITCH, PITCH, d * 16, li, g);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[mt][d] = Y::mma(vt, p[mt][kk], o[mt][d]);
+            }
+        cur ^= 1;
+        on_next = live.bits(mask != nullptr, len, (tile + 1) * 64, lane);
+        nxt.put(lds + cur * 2 * Tile::TILE, lds + cur * 2 * Tile::TILE + Tile::TILE, on_next);
+        on = on_next;
+        load(tile + 2);
+        __syncthreads();
+    }
+
+    const size_t rows = (size_t)a.B * a.Hkv * a.M;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const float l = groups_sum(sum[mt]), top = mx[mt];
+        const int m = m0 + mt * 16 + li;
+        if (m >= a.M) continue;
+        const size_t at_row = (size_t)split * rows + (size_t)pair * a.M + m;
+        const float inv = a.nsplit > 1 ? 1.f : top == -INFINITY ? 0.f : 1.f / l;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const int col = d * 16 + g * 4;
+            if (col >= a.D) continue;
+            if (a.nsplit == 1) store_out(a, row_at(a, b, hk, m) + col, o[mt][d] * inv);
+            else *reinterpret_cast<f32x4*>(a.ws + at_row * a.D + col) = o[mt][d];
+        }
+        if (g == 0) {
+            if (a.nsplit > 1) {
+                float* st = a.ws + (size_t)a.nsplit * rows * a.D + at_row * 2;
+                st[0] = top;
+                st[1] = l;
+            } else if (a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(l)) * LN2;
+        }
+    }
+}
+
+// the rows' side of the backward, the same way
+template <int DF, int NW>
+__global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
+    typedef Ty<bf16_t> Y;
+    typedef RowTile<DF, NW> Tile;
+    constexpr int DT = DF * 2, PITCH = Tile::PITCH, MT = 2;
+    __shared__ __attribute__((aligned(16))) char lds[4 * Tile::TILE];
+    const int wi = work_item(a.blocks);
+    if (wi >= a.blocks) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int rb = wi % a.row_blocks, pair = wi / a.row_blocks, b = pair / a.Hkv, hk = pair % a.Hkv, m0 = (rb * NW + wave) * 16 * MT;
+    const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
+    const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
+    const bf16_t* kb = a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh;
+    const bf16_t* vb = a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh;
+    const int last = (len + 63) / 64;
+    const size_t out0 = row_at(a, b, hk, 0);
+
+    bf16x8_t q[MT][DF], d_o[MT][DF];
+    float lse[MT], delta[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int m = m0 + mt * 16 + li;
+        load_rows<bf16_t, DF>(a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh, a.q_st, a.q_sh, m, a.M, a.G, a.D, g, q[mt]);
+        load_rows<bf16_t, DF>(a.dout + out0, (long)a.H * a.D, a.D, m, a.M, a.G, a.D, g, d_o[mt]);
+        const size_t at = stat_at(a, b, hk, min(m, a.M - 1));
+        const float l = a.lse[at];
+        delta[mt] = a.delta[at];
+        lse[mt] = m < a.M ? l * LOG2E : INFINITY;
+    }
+    Tile nxt;
+    Live64 live;
+    nxt.init(a.D);
+    auto load = [&](int tile) {
+        const int key0 = tile * 64, rows = min(64, len - key0);
+        live.load(mask, kb, key0, a.Tk, lane);
+        const Window kw = Tile::window(kb, a.k_st, key0, rows, a.D), vw = Tile::window(vb, a.v_st, key0, rows, a.D);
+#pragma unroll
+        for (int i = 0; i < Tile::NI; ++i) {
+            nxt.x[i] = kw.load((nxt.row(i) * (unsigned)a.k_st + nxt.col(i)) * 2u);
+            nxt.y[i] = vw.load((nxt.row(i) * (unsigned)a.v_st + nxt.col(i)) * 2u);
+        }
+    };
+    load(0);
+    f32x4 dq[MT][DT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dq[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float scale2 = a.scale * LOG2E;
+    if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
+    unsigned long long on = live.bits(mask != nullptr, len, 0, lane);
+    nxt.put(lds, lds + Tile::TILE, on);
+    load(1);
+    __syncthreads();
+
+    int cur = 0;
+    for (int tile = 0; tile < last; ++tile) {
+        const char *lk = lds + cur * 2 * Tile::TILE, *lv = lk + Tile::TILE;
+        const bool full = on == ~0ull;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            Y::half h[MT][2];
+#pragma unroll
+            for (int ns = 0; ns < 2; ++ns) {
+                const int sub = kk * 2 + ns;
+                f32x4 s[MT], dp[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt] = dp[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int f = 0; f < DF; ++f) {
+                    const bf16x8_t k = frag_at<bf16_t>(lk, PITCH, sub * 16 + li, f, g), v = frag_at<bf16_t>(lv, PITCH, sub * 16 + li, f, g);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        s[mt] = Y::mma(k, q[mt][f], s[mt]);
+                        dp[mt] = Y::mma(v, d_o[mt][f], dp[mt]);
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float ds = __builtin_amdgcn_exp2f(s[mt][r] * scale2 - lse[mt]) * (dp[mt][r] - delta[mt]);
+                        if (!full) ds = (on >> (sub * 16 + g * 4 + r)) & 1 ? ds : 0.f;
+                        dp[mt][r] = ds;
+                    }
+                    h[mt][ns] = Y::pack(dp[mt]);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const bf16x8_t kt = frag_t<bf16_t>(lk + kk * 32 * PITCH, PITCH, d * 16, li, g);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) dq[mt][d] = Y::mma(kt, Y::join(h[mt]), dq[mt][d]);
+            }
+        }
+        cur ^= 1;
+        on = live.bits(mask != nullptr, len, (tile + 1) * 64, lane);
+        nxt.put(lds + cur * 2 * Tile::TILE, lds + cur * 2 * Tile::TILE + Tile::TILE, on);
+        load(tile + 2);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int m = m0 + mt * 16 + li;
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const int col = d * 16 + g * 4;
+            if (col < a.D) store4(a.dq + row_at(a, b, hk, m) + col, dq[mt][d] * a.scale);
+        }
+    }
+}
+
+// the keys' side: a wave keeps 32 keys, their rows and both gradients in registers, q and dO pass through LDS R
+// rows at a time
+template <int DF, int NW>
+__global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
+    typedef Ty<bf16_t> Y;
+    constexpr int R = DF == 4 ? 32 : 64;                     // (at the widest rows a prefetch of 64 would not fit the registers)
+    typedef RowTile<DF, NW, R> Tile;
+    constexpr int DT = DF * 2, PITCH = Tile::PITCH;
+    __shared__ __attribute__((aligned(16))) char lds[4 * Tile::TILE];
+    __shared__ __attribute__((aligned(16))) float l_lse[2][R], l_delta[2][R];
+    const int wi = work_item(a.blocks);
+    if (wi >= a.blocks) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int kblocks = a.row_blocks, kbk = wi % kblocks, pair = wi / kblocks, b = pair / a.Hkv, hk = pair % a.Hkv;
+    const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
+    const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
+    const int key0 = (kbk * NW + wave) * 32, block0 = kbk * NW * 32;
+    const float scale2 = a.scale * LOG2E;
+    const bf16_t* qb = a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh;
+    const bf16_t* dob = a.dout + row_at(a, b, hk, 0);
+
+    const KeyBits<bf16_t> bits = key_bits(a, mask, len, key0, li);
+    bf16x8_t k[2][DF], v[2][DF];
+    load_keys<bf16_t, DF>(a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh, a.k_st, bits, key0, a.D, li, g, k);
+    load_keys<bf16_t, DF>(a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh, a.v_st, bits, key0, a.D, li, g, v);
+    f32x4 dk[2][DT], dv[2][DT];
+#pragma unroll
+    for (int ns = 0; ns < 2; ++ns)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dk[ns][d] = dv[ns][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (block0 < len) {                                      // (a block behind the regions: its gradients are zero)
+        Tile nxt;
+        float n_lse, n_delta;
+        nxt.init(a.D);
+        auto load = [&](int m0) {                            // rows past the last one repeat it; their p is zero
+#pragma unroll
+            for (int i = 0; i < Tile::NI; ++i) {
+                const int m = min(m0 + (int)nxt.row(i), a.M - 1), t = m / a.G, hh = m - t * a.G;
+                nxt.x[i] = *reinterpret_cast<const u32x4*>(qb + (size_t)t * a.q_st + (size_t)hh * a.q_sh + nxt.col(i));
+                nxt.y[i] = *reinterpret_cast<const u32x4*>(dob + ((size_t)t * a.H + hh) * a.D + nxt.col(i));
+            }
+            const int m = m0 + (lane & (R - 1));
+            const size_t at = stat_at(a, b, hk, min(m, a.M - 1));
+            const float l = a.lse[at];
+            n_delta = a.delta[at];
+            n_lse = m < a.M ? l * LOG2E : INFINITY;
+        };
+        auto put = [&](int buf) {
+            nxt.put(lds + buf * 2 * Tile::TILE, lds + buf * 2 * Tile::TILE + Tile::TILE, ~0ull);
+            if (wave == 0 && lane < R) { l_lse[buf][lane] = n_lse; l_delta[buf][lane] = n_delta; }
+        };
+        load(0);
+        if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
+        put(0);
+        load(R);
+        __syncthreads();
+        int cur = 0;
+        for (int m0 = 0; m0 < a.M; m0 += R) {
+            const char *lq = lds + cur * 2 * Tile::TILE, *ldo = lq + Tile::TILE;
+#pragma unroll
+            for (int hf = 0; hf < R / 32; ++hf) {
+                Y::half p[2][2], ds[2][2];                   // [key tile][row tile]
+#pragma unroll
+                for (int qs = 0; qs < 2; ++qs) {
+                    const int row = hf * 32 + qs * 16;
+                    f32x4 s[2], dp[2];
+#pragma unroll
+                    for (int ns = 0; ns < 2; ++ns) s[ns] = dp[ns] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int f = 0; f < DF; ++f) {
+                        const bf16x8_t qf = frag_at<bf16_t>(lq, PITCH, row + li, f, g), df = frag_at<bf16_t>(ldo, PITCH, row + li, f, g);
+#pragma unroll
+                        for (int ns = 0; ns < 2; ++ns) {
+                            s[ns] = Y::mma(qf, k[ns][f], s[ns]);
+                            dp[ns] = Y::mma(df, v[ns][f], dp[ns]);
+                        }
+                    }
+                    const f32x4 ls = *reinterpret_cast<const f32x4*>(&l_lse[cur][row + g * 4]);
+                    const f32x4 de = *reinterpret_cast<const f32x4*>(&l_delta[cur][row + g * 4]);
+#pragma unroll
+                    for (int ns = 0; ns < 2; ++ns) {
+                        const bool on = (bits.b[ns] >> li) & 1;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            s[ns][r] = on ? __builtin_amdgcn_exp2f(s[ns][r] * scale2 - ls[r]) : 0.f;
+                            dp[ns][r] = s[ns][r] * (dp[ns][r] - de[r]);
+                        }
+                        p[ns][qs] = Y::pack(s[ns]);
+                        ds[ns][qs] = Y::pack(dp[ns]);
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const bf16x8_t dot_ = frag_t<bf16_t>(ldo + hf * 32 * PITCH, PITCH, d * 16, li, g);
+                    const bf16x8_t qt = frag_t<bf16_t>(lq + hf * 32 * PITCH, PITCH, d * 16, li, g);
+#pragma unroll
+                    for (int ns = 0; ns < 2; ++ns) {
+                        dv[ns][d] = Y::mma(dot_, Y::join(p[ns]), dv[ns][d]);
+                        dk[ns][d] = Y::mma(qt, Y::join(ds[ns]), dk[ns][d]);
+                    }
+                }
+            }
+            cur ^= 1;
+            put(cur);
+            load(m0 + 2 * R);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int ns = 0; ns < 2; ++ns) {
+        const int key = key0 + ns * 16 + li;
+        if (key >= a.Tk) continue;
+        const size_t at = (((size_t)b * a.Tk + key) * a.Hkv + hk) * a.D;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const int c = d * 16 + g * 4;
+            if (c < a.D) {
+                store4(a.dk + at + c, dk[ns][d] * a.scale);
+                store4(a.dv + at + c, dv[ns][d]);
+            }
+        }
+    }
+}
+
 // ---- host -----------------------------------------------------------------------------------
 int key_tile(int dtype) { return dtype == VQA_BF16 ? 32 : 16; }
 
 // 16-row tiles a workgroup of the forward takes: all of a pair's rows up to 64 (each further tile re-reads the keys from
-// the caches, not from registers); fp32 holds half as many
-int row_tiles(long M, int dtype) {
-    const int most = dtype == VQA_BF16 ? 4 : 2;
+// the caches, not from registers); fp32, and rows wider than 96,
+// leave registers for half as many
+int row_tiles(long M, int D, int dtype) {
+    const int most = dtype == VQA_BF16 && D <= 96 ? 4 : 2;
     int mt = 1;
     while (mt < most && 16L * mt < M) mt *= 2;
     return mt;
 }
-// Key ranges: one when the work items fill the chip; otherwise as many as bring 1024 of them, of at least 8 key tiles each
-// (two per wave), and at most 32 (the join reads them one after the other).
-int key_splits(long items, int Tk, int dtype) {
-    const int tiles = (Tk + key_tile(dtype) - 1) / key_tile(dtype);
-    if (items >= 512 || tiles < 16) return 1;
-    long n = (1024 + items - 1) / items;
-    if (n > tiles / 8) n = tiles / 8;
+// Key ranges: one when the work items fill the chip (two to a CU, one where a workgroup fills it); otherwise as many as bring
+// twice that, of at least 256 keys each (bf16; 128 fp32), and at most 32 (the join reads them one after the other).
+int key_splits(long items, int Tk, int dtype, bool tiled) {
+    const int tile = tiled ? 64 : key_tile(dtype), tiles = (Tk + tile - 1) / tile, least = tiled ? 4 : 8;
+    const long fill = tiled ? 256 : 512;
+    if (items >= fill || tiles < 2 * least) return 1;
+    long n = (2 * fill + items - 1) / items;
+    if (n > tiles / least) n = tiles / least;
     if (n > 32) n = 32;
     const int per = (int)((tiles + n - 1) / n);
     return (tiles + per - 1) / per;                          // no empty range
 }
 bool one_pass(long M) { return M <= 32; }                    // the backward that keeps all rows of a pair on the chip
+bool tiled(long M, int Tk, int dtype) { return dtype == VQA_BF16 && M > 64 && Tk > 256; }        // k_xattn_*_tile
+// Waves of a tiled workgroup: eight share a key tile; four for so few rows that they take no more
+int tile_waves(long M) { return M <= 128 ? 4 : 8; }
 
-int fwd_splits(int B, int Tq, int Tk, int H, int Hkv, int dtype) {
-    const long M = (long)Tq * (H / Hkv), mt = row_tiles(M, dtype);
-    return key_splits((long)B * Hkv * ((M + 16 * mt - 1) / (16 * mt)), Tk, dtype);
+int fwd_splits(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
+    const long M = (long)Tq * (H / Hkv), mt = row_tiles(M, D, dtype), rows = tiled(M, Tk, dtype) ? 32 * tile_waves(M) : 16 * mt;
+    return key_splits((long)B * Hkv * ((M + rows - 1) / rows), Tk, dtype, tiled(M, Tk, dtype));
 }
-int bwd_splits(int B, int Tq, int Tk, int H, int Hkv, int dtype) { return key_splits((long)B * Hkv, Tk, dtype); }
+int bwd_splits(int B, int Tq, int Tk, int H, int Hkv, int dtype) { return key_splits((long)B * Hkv, Tk, dtype, false); }
 
 // Waves per work item: two, so that an item's end (the join) and the next one's beginning overlap with other items; four
 // where the items are fewer than two to a CU and only their own length counts (one image of 196 regions: 5.6 against 7.2 us,
@@ -1004,7 +1456,7 @@ template <typename T, int DF, int MT> void launch_fwd(const Args<T>& a, hipStrea
 template <typename T, int DF> void launch_fwd_mt(const Args<T>& a, int mt, hipStream_t s) {
     if (mt == 1) launch_fwd<T, DF, 1>(a, s);
     else if (mt == 2) launch_fwd<T, DF, 2>(a, s);
-    else if constexpr (sizeof(T) == 2) launch_fwd<T, DF, 4>(a, s);
+    else if constexpr (sizeof(T) == 2 && DF < 4) launch_fwd<T, DF, 4>(a, s);
 }
 template <typename T, int DF> void launch_bwd(const Args<T>& a, hipStream_t s) {
     const int grid = 8 * ((a.blocks + 7) / 8);
@@ -1063,16 +1515,40 @@ Args<T> args_of(const VqaAttnView& q, const VqaAttnView& k, const VqaAttnView& v
     return a;
 }
 
+// f<DF> for the tiled kernels
+#define TILED(D, call)                                                                         \
+    switch (((D) + 31) / 32) {                                                                 \
+        case 1: { constexpr int DF = 1; call; break; }                                         \
+        case 2: { constexpr int DF = 2; call; break; }                                         \
+        case 3: { constexpr int DF = 3; call; break; }                                         \
+        default: { constexpr int DF = 4; call; break; }                                        \
+    }
+
 template <typename T>
 int fwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
-    const int mt = row_tiles(a.M, dtype);
-    a.row_blocks = (a.M + 16 * mt - 1) / (16 * mt);
     a.nsplit = nsplit;
-    const int tiles = (a.Tk + Ty<T>::KC - 1) / Ty<T>::KC;
-    a.tiles_split = (tiles + nsplit - 1) / nsplit;
-    a.items = a.B * a.Hkv * a.row_blocks * nsplit;
-    a.blocks = waves_of(a.items) == 2 ? (a.items + 1) / 2 : a.items;
-    BY_WIDTH(T, a.D, (launch_fwd_mt<T, DF>(a, mt, stream)));
+    bool done = false;
+    if constexpr (sizeof(T) == 2) {
+        if (tiled(a.M, a.Tk, dtype)) {
+            const int nw = tile_waves(a.M), tiles = (a.Tk + 63) / 64;
+            a.row_blocks = (a.M + 32 * nw - 1) / (32 * nw);
+            a.tiles_split = (tiles + nsplit - 1) / nsplit;
+            a.blocks = a.B * a.Hkv * a.row_blocks * nsplit;
+            const int grid = 8 * ((a.blocks + 7) / 8);
+            if (nw == 8) { TILED(a.D, (k_xattn_fwd_tile<DF, 8><<<grid, 512, 0, stream>>>(a))) }
+            else { TILED(a.D, (k_xattn_fwd_tile<DF, 4><<<grid, 256, 0, stream>>>(a))) }
+            done = true;
+        }
+    }
+    if (!done) {
+        const int mt = row_tiles(a.M, a.D, dtype);
+        a.row_blocks = (a.M + 16 * mt - 1) / (16 * mt);
+        const int tiles = (a.Tk + Ty<T>::KC - 1) / Ty<T>::KC;
+        a.tiles_split = (tiles + nsplit - 1) / nsplit;
+        a.items = a.B * a.Hkv * a.row_blocks * nsplit;
+        a.blocks = waves_of(a.items) == 2 ? (a.items + 1) / 2 : a.items;
+        BY_WIDTH(T, a.D, (launch_fwd_mt<T, DF>(a, mt, stream)));
+    }
     int rc = vqa_check_launch("vqa_cross_attn_fwd");
     if (rc || nsplit == 1) return rc;
     const size_t n = (size_t)a.B * a.Hkv * a.M * (a.D / 4);
@@ -1081,7 +1557,7 @@ int fwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
 }
 
 template <typename T>
-int bwd(Args<T> a, int nsplit, hipStream_t stream) {
+int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
     if (one_pass(a.M)) {
         a.nsplit = nsplit;
         const int tiles = (a.Tk + Ty<T>::KC - 1) / Ty<T>::KC;
@@ -1098,6 +1574,21 @@ int bwd(Args<T> a, int nsplit, hipStream_t stream) {
     const size_t rows = (size_t)a.B * a.Tq * a.H;
     k_xattn_delta<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(a, a.ws);
     a.delta = a.ws;
+    if constexpr (sizeof(T) == 2) {
+        if (tiled(a.M, a.Tk, dtype)) {
+            const int nw = tile_waves(a.M);
+            a.row_blocks = (a.M + 32 * nw - 1) / (32 * nw);
+            a.blocks = a.B * a.Hkv * a.row_blocks;
+            int grid = 8 * ((a.blocks + 7) / 8);
+            if (nw == 8) { TILED(a.D, (k_xattn_bwd_q_tile<DF, 8><<<grid, 512, 0, stream>>>(a))) }
+            else { TILED(a.D, (k_xattn_bwd_q_tile<DF, 4><<<grid, 256, 0, stream>>>(a))) }
+            a.row_blocks = (a.Tk + 255) / 256;
+            a.blocks = a.B * a.Hkv * a.row_blocks;
+            grid = 8 * ((a.blocks + 7) / 8);
+            TILED(a.D, (k_xattn_bwd_kv_tile<DF, 8><<<grid, 512, 0, stream>>>(a)))
+            return vqa_check_launch("vqa_cross_attn_bwd");
+        }
+    }
     BY_WIDTH(T, a.D, (launch_bwd_two<T, DF>(a, stream)));
     return vqa_check_launch("vqa_cross_attn_bwd");
 }
@@ -1120,7 +1611,7 @@ extern "C" {
 
 size_t vqa_cross_attn_fwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
     if (!sizes_ok(B, Tq, Tk, H, Hkv, D, dtype)) return 0;
-    const int n = fwd_splits(B, Tq, Tk, H, Hkv, dtype);
+    const int n = fwd_splits(B, Tq, Tk, H, Hkv, D, dtype);
     return n > 1 ? (size_t)n * B * Tq * H * (D + 2) : 0;
 }
 size_t vqa_cross_attn_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
@@ -1134,7 +1625,7 @@ int vqa_cross_attn_fwd(const VqaAttnView* q, const VqaAttnView* k, const VqaAttn
                        long mask_sb, float scale, void* o, void* o_rest, float* lse, float* workspace, int B, int Tq, int Tk, int H, int Hkv,
                        int D, int dtype, hipStream_t stream) {
     XA_COMMON("vqa_cross_attn_fwd")
-    const int n = fwd_splits(B, Tq, Tk, H, Hkv, dtype);
+    const int n = fwd_splits(B, Tq, Tk, H, Hkv, D, dtype);
     VQA_REQUIRE(o && aligned16(o) && aligned16(o_rest) && aligned16(workspace) && (workspace || n == 1),
                 "vqa_cross_attn_fwd: o must be 16-byte aligned; this size needs the workspace");
     if (dtype == VQA_BF16) {
@@ -1159,12 +1650,12 @@ int vqa_cross_attn_bwd(const void* d_o, const VqaAttnView* q, const VqaAttnView*
         Args<bf16_t> a = args_of<bf16_t>(*q, *k, *v, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D);
         a.dout = (const bf16_t*)d_o; a.o = (bf16_t*)o; a.rest = (bf16_t*)o_rest; a.lse = (float*)lse;
         a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv; a.ws = workspace;
-        return bwd(a, n, stream);
+        return bwd(a, n, dtype, stream);
     }
     Args<float> a = args_of<float>(*q, *k, *v, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D);
     a.dout = (const float*)d_o; a.o = (float*)o; a.lse = (float*)lse;
     a.dq = (float*)dq; a.dk = (float*)dk; a.dv = (float*)dv; a.ws = workspace;
-    return bwd(a, n, stream);
+    return bwd(a, n, dtype, stream);
 }
 
 }  // extern "C"
