@@ -443,7 +443,7 @@ int vqa_gated_scan_bwd(const void* dh, const float* dc_last, const void* gates, 
 /* Cross attention of Tq token rows to Tk region rows, H query heads on Hkv key heads (head h reads key head h / (H / Hkv)):
  *   o[b,t,h] = sum_r p_r v[b,r],  p = softmax_r(scale * q[b,t,h].k[b,r])  over the regions r < kv_len[b] with mask[b,r] != 0
  *   q (B, Tq, H, D), k and v (B, Tk, Hkv, D) are views: row (b, t, h) at data + b * sb + t * st + h * sh (elements,
- *               multiples of 8, st < 2^26), D contiguous
+ *               multiples of 8, st < 2^25), D contiguous
  *   kv_len      optional (B), clamped to [0, Tk]; mask optional bytes, row b at mask + b * mask_sb.  What rows of k and v
  *               that do not count hold, NaN included, has no effect, and their gradients are 0
  *   o           (B, Tq, H, D) contiguous; a row with no region that counts is 0
@@ -455,7 +455,7 @@ int vqa_gated_scan_bwd(const void* dh, const float* dc_last, const void* gates, 
  * regions are split over workgroups where the batch does not fill the chip.
  * Backward: d_o as o; dq as o, dk and dv (B, Tk, Hkv, D) contiguous, summed over the heads that share a key head.
  * Scores, softmax and sums are fp32; with bf16 storage p and its gradient are rounded to bf16 for the products.
- * D % 8 == 0, D <= VQA_CROSS_ATTN_MAX_D, B * Tq * H <= 2^27, Tk <= 2^24, Hkv * D < 2^26. */
+ * D % 8 == 0, D <= VQA_CROSS_ATTN_MAX_D, B * Tq * H <= 2^27, Tk <= 2^24, Hkv * D < 2^25. */
 #define VQA_CROSS_ATTN_MAX_D 128
 typedef struct VqaAttnView { const void* data; long sb, st, sh; } VqaAttnView;
 size_t vqa_cross_attn_fwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype);

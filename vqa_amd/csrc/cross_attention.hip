@@ -1420,13 +1420,12 @@ int row_tiles(long M, int D, int dtype) {
     while (mt < most && 16L * mt < M) mt *= 2;
     return mt;
 }
-// Key ranges: one when the work items fill the chip (two to a CU, one where a workgroup fills it); otherwise as many as bring
-// twice that, of at least 256 keys each (bf16; 128 fp32), and at most 32 (the join reads them one after the other).
+// Key ranges: one when the work items give every CU one; otherwise as many as bring two to a CU, of at least 256 keys each
+// (bf16; 128 fp32), and at most 32 (the join reads them one after the other).
 int key_splits(long items, int Tk, int dtype, bool tiled) {
     const int tile = tiled ? 64 : key_tile(dtype), tiles = (Tk + tile - 1) / tile, least = tiled ? 4 : 8;
-    const long fill = tiled ? 256 : 512;
-    if (items >= fill || tiles < 2 * least) return 1;
-    long n = (2 * fill + items - 1) / items;
+    if (items >= 256 || tiles < 2 * least) return 1;
+    long n = (512 + items - 1) / items;
     if (n > tiles / least) n = tiles / least;
     if (n > 32) n = 32;
     const int per = (int)((tiles + n - 1) / n);
@@ -1500,7 +1499,7 @@ template <typename T, int DF> void launch_bwd_two(Args<T> a, hipStream_t s) {
     } while (0)
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-bool view_ok(const VqaAttnView& v) { return v.data && aligned16(v.data) && v.sb % 8 == 0 && v.st % 8 == 0 && v.sh % 8 == 0 && v.sb >= 0 && v.st >= 0 && v.sh >= 0 && v.st < (1L << 26); }
+bool view_ok(const VqaAttnView& v) { return v.data && aligned16(v.data) && v.sb % 8 == 0 && v.st % 8 == 0 && v.sh % 8 == 0 && v.sb >= 0 && v.st >= 0 && v.sh >= 0 && v.st < (1L << 25); }
 
 template <typename T>
 Args<T> args_of(const VqaAttnView& q, const VqaAttnView& k, const VqaAttnView& v, const int32_t* kv_len, const uint8_t* mask,
@@ -1596,7 +1595,7 @@ int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
 bool sizes_ok(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
     return (dtype == VQA_F32 || dtype == VQA_BF16) && B > 0 && Tq > 0 && Tk > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && D > 0 &&
            D % 8 == 0 && D <= VQA_CROSS_ATTN_MAX_D && (long)B * Tq * H <= (1L << 27) && Tk <= (1 << 24) &&
-           (long)B * Hkv * ((Tk + 63) / 64) <= (1L << 28) && (long)Hkv * D < (1L << 26);
+           (long)B * Hkv * ((Tk + 63) / 64) <= (1L << 28) && (long)Hkv * D < (1L << 25);
 }
 #define XA_COMMON(fn)                                                                                                          \
     VQA_REQUIRE(sizes_ok(B, Tq, Tk, H, Hkv, D, dtype), fn ": dtype VQA_F32 or VQA_BF16, positive sizes, H a multiple of Hkv, " \

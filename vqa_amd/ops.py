@@ -58,23 +58,21 @@ def _need(cond, msg, *args):
 def _storage(name, t):
     if not t.is_cuda:
         raise VqaHipError(f'{name} runs on a HIP device only (inputs must be cuda tensors); there is no CPU path')
-    return _lib.dtype_code(t.dtype)
+    return _lib.BF16 if t.dtype is torch.bfloat16 else _lib.dtype_code(t.dtype)
 
 
 def _like(name, what, t, ref, shape, dtype=None):
     """`t` checked against the operand `ref` it goes with."""
-    if t.shape != shape or t.dtype != (dtype or ref.dtype) or t.device != ref.device:
+    if t.shape != shape or t.dtype is not (dtype or ref.dtype) or t.get_device() != ref.get_device():
         raise ValueError(f'{name}: {what} must be {tuple(shape)} {dtype or ref.dtype} on {ref.device}, '
                          f'got {tuple(t.shape)} {t.dtype} on {t.device}')
 
 
 def _packed(t):
     """`t`, contiguous and 16-byte aligned."""
-    if t is None:
-        return None
-    if not t.is_contiguous():
-        t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _lengths(name, what, t, ref, n):
@@ -314,7 +312,7 @@ def _view(t):
     sb, st, sh, one = t.stride()
     nb, nt, nh, D = t.shape                                      # the stride of a size of 1 says nothing
     sb, st, sh = sb if nb > 1 else 0, st if nt > 1 else 0, sh if nh > 1 else 0
-    if one != 1 or (sb | st | sh) % 8 or sb < 0 or st < 0 or sh < 0 or st >= 1 << 26 or t.data_ptr() % 16:
+    if one != 1 or (sb | st | sh) % 8 or sb < 0 or st < 0 or sh < 0 or st >= 1 << 25 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
         sb, st, sh, one = t.stride()
     return t, _lib.AttnView(t.data_ptr(), sb, st, sh)
