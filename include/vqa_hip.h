@@ -425,14 +425,14 @@ int vqa_cast_pad(const float* src, int ld_src, void* dst, int ld_dst, int M, int
  *   c0       optional (B, H) fp32 starting state (0 when NULL); c_last optional (B, H) fp32: the state after the last
  *            step, so that a call with T = 1 is one step of a running sequence
  *   h        (B, T, H)
- *   saved    vqa_gated_scan_saved_floats fp32 (states every VQA_GATED_SCAN_SAVE steps) for the backward; NULL when none
+ *   saved    vqa_gated_scan_saved_floats fp32 (the states in front of steps 0, SAVE, 2 SAVE, ...) for the backward; NULL when none
  *            follows
  *   workspace  vqa_gated_scan_workspace_floats fp32 (may be 0: NULL), scratch of one call
  * Backward: dh (B, T, H) and dc_last (B, H) fp32, either NULL when it is zero; writes dgates (B, T, 4H) and, unless
  * NULL, dc0 (B, H) fp32.  H % 8 == 0, T <= VQA_GATED_SCAN_MAX_T, B * H <= 2^30. */
 #define VQA_GATED_SCAN_SAVE 8
 #define VQA_GATED_SCAN_MAX_T (1 << 20)
-size_t vqa_gated_scan_workspace_floats(int B, int T, int H);
+size_t vqa_gated_scan_workspace_floats(int B, int T, int H, int dtype);
 size_t vqa_gated_scan_saved_floats(int B, int T, int H);
 int vqa_gated_scan_fwd(const void* gates, long sb, long st, const int32_t* lengths, const float* c0, void* h, float* c_last,
                        float* saved, float* workspace, int B, int T, int H, int dtype, hipStream_t stream);

@@ -39,8 +39,8 @@ def test_scan_forward_refuses(change):
 
 
 def test_scan_backward_refuses():
-    ok = dict(dh=P, dc=P, gates=P, sb=64, st=32, lengths=None, c0=None, saved=None, dgates=P, dc0=P, ws=None, B=2, T=2, H=8, dtype=0)
-    for change in (dict(dh=None, dc=None), dict(dgates=None), dict(dh=P + 4), dict(saved=P + 4), dict(T=9), dict(dtype=3), dict(gates=0)):
+    ok = dict(dh=P, dc=P, gates=P, sb=64, st=32, lengths=None, c0=None, saved=P, dgates=P, dc0=P, ws=None, B=2, T=2, H=8, dtype=0)
+    for change in (dict(dh=None, dc=None), dict(dgates=None), dict(dh=P + 4), dict(saved=P + 4), dict(saved=None), dict(dtype=3), dict(gates=0)):
         refused('vqa_gated_scan_bwd', *{**ok, **change}.values())
 
 
@@ -89,8 +89,8 @@ def test_attention_backward_refuses():
 
 def test_workspace_sizes():
     lib = _lib.load()
-    assert lib.vqa_gated_scan_workspace_floats(256, 14, 2400) == 0 and lib.vqa_gated_scan_workspace_floats(1, 4096, 512) > 0
-    assert lib.vqa_gated_scan_saved_floats(2, 17, 8) == 2 * 2 * 8 and lib.vqa_gated_scan_saved_floats(2, 1, 8) == 0
+    assert lib.vqa_gated_scan_workspace_floats(256, 14, 2400, 1) == 0 and lib.vqa_gated_scan_workspace_floats(1, 4096, 512, 1) > 0
+    assert lib.vqa_gated_scan_saved_floats(2, 17, 8) == 3 * 2 * 8 and lib.vqa_gated_scan_saved_floats(2, 1, 8) == 2 * 8
     assert lib.vqa_norm_gate_workspace_floats(100, 64, 0) >= 3 * 64 and lib.vqa_norm_gate_workspace_floats(100, 64, 7) == 0
     assert lib.vqa_cross_attn_fwd_workspace_floats(256, 14, 196, 15, 15, 80, 1) == 0
     assert lib.vqa_cross_attn_fwd_workspace_floats(1, 1, 4096, 8, 2, 64, 1) > 0

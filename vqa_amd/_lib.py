@@ -83,7 +83,7 @@ _SIGNATURES = {
     'vqa_tanh_dropout_bwd': [_p, _i, _z, _p, _i, _p, _i, _i, _i, _u, _f, _i, _p],
     'vqa_colsum': [_p, _i, _p, _i, _i, _i, _p],
     'vqa_cast_pad': [_p, _i, _p, _i, _i, _i, _i, _p],
-    'vqa_gated_scan_workspace_floats': [_i, _i, _i],
+    'vqa_gated_scan_workspace_floats': [_i, _i, _i, _i],
     'vqa_gated_scan_saved_floats': [_i, _i, _i],
     'vqa_gated_scan_fwd': [_p, _l, _l, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     'vqa_gated_scan_bwd': [_p, _p, _p, _l, _l, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],

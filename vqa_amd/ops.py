@@ -112,12 +112,12 @@ def gated_scan_fwd(gates, lengths=None, c0=None, save=True):
     dev = gates.device
     h = torch.empty((B, T, H), dtype=gates.dtype, device=dev)
     c = torch.empty((B, H), dtype=torch.float32, device=dev)
-    saved = torch.empty(((T - 1) // _SAVE if T else 0, B, H), dtype=torch.float32, device=dev) if save else None
+    saved = torch.empty(((T + _SAVE - 1) // _SAVE, B, H), dtype=torch.float32, device=dev) if save else None
     if B == 0 or T == 0 or H == 0:
         return h, c.zero_() if c0 is None else c.copy_(c0), saved
-    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H), dev)
+    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H, dt), dev)
     _call(dev, 'vqa_gated_scan_fwd', gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0), h.data_ptr(), c.data_ptr(),
-          saved.data_ptr() if save and T > _SAVE else None, _ptr(ws), B, T, H, dt)
+          _ptr(saved), _ptr(ws), B, T, H, dt)
     return h, c, saved
 
 
@@ -136,11 +136,11 @@ def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
         dc = _packed(dc)
     if B == 0 or T == 0 or H == 0 or (dh is None and dc is None):
         return dgates.zero_(), dc0.zero_() if dc is None else dc0.copy_(dc)
-    _need(saved is not None and tuple(saved.shape) == ((T - 1) // _SAVE, B, H),
+    _need(saved is not None and tuple(saved.shape) == ((T + _SAVE - 1) // _SAVE, B, H),
           'gated_scan: the backward needs what gated_scan_fwd(..., save=True) returned for these gates')
-    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H), dev)
+    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H, dt), dev)
     _call(dev, 'vqa_gated_scan_bwd', _ptr(dh), _ptr(dc), gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0),
-          saved.data_ptr() if T > _SAVE else None, dgates.data_ptr(), dc0.data_ptr(), _ptr(ws), B, T, H, dt)
+          saved.data_ptr(), dgates.data_ptr(), dc0.data_ptr(), _ptr(ws), B, T, H, dt)
     return dgates, dc0
 
 
