@@ -83,7 +83,7 @@ def test_attention_backward_refuses():
     ok = dict(do=P, q=view(), k=view(), v=view(), o=P, rest=None, lse=P, kv_len=None, mask=None, mask_sb=0, scale=0.25, dq=P, dk=P, dv=P, ws=P, B=2,
               Tq=3, Tk=16, H=4, Hkv=2, D=16, dtype=1)
     for change in (dict(do=None), dict(o=None), dict(lse=None), dict(dq=None), dict(dk=P + 4), dict(dv=None), dict(D=10), dict(v=view(st=4)),
-                   dict(Tq=40, ws=None), dict(ws=P + 4), dict(rest=P + 4)):
+                   dict(Tq=40, Tk=64, ws=None), dict(ws=P + 4), dict(rest=P + 4)):
         refused('vqa_cross_attn_bwd', *{**ok, **change}.values())
 
 

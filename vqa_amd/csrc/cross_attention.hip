@@ -968,6 +968,271 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_kv(Args<T> a) {
     }
 }
 
+// ---- few keys -------------------------------------------------------------------------------
+// At most 32 keys under more than 32 rows: the roles change.  The keys and values of a pair (NK tiles of 16) stay in every
+// wave's registers, the rows stream past, 16 at a time and each read once; scores of a row are complete at once, so the
+// softmax needs no second look; dq leaves with its rows, dk and dv are summed in registers over a wave's rows and joined
+// over waves and row ranges at the end.
+template <typename T, int DF, int NK> struct FewKeys {
+    typedef Ty<T> Y;
+    static constexpr int DP = DF * Y::KC, DT = DP / 16, PITCH = DP * (int)sizeof(T) + Y::PAD, TILE = 16 * PITCH;
+    // one operand's keys to LDS (zeros for those that do not count)
+    static __device__ __forceinline__ void stage(char* lds, const T* base, long st, unsigned on, int Tk, int D) {
+        constexpr int CH = DP / Y::E;
+        for (int c = threadIdx.x; c < 16 * NK * CH; c += blockDim.x) {
+            const int r = c / CH, col = (c % CH) * Y::E;
+            typename Y::frag x = {};
+            if (((on >> r) & 1) && col < D) x = *reinterpret_cast<const typename Y::frag*>(base + (size_t)r * st + col);
+            *reinterpret_cast<typename Y::frag*>(lds + r * PITCH + col * (int)sizeof(T)) = x;
+        }
+    }
+    static __device__ __forceinline__ unsigned live(const Args<T>& a, const uint8_t* mask, int len, int lane) {
+        const int key = lane & 31;
+        return (unsigned)(__ballot(key < 16 * NK && key < len && (!mask || mask[key] != 0)) & 0xffffffffu);
+    }
+};
+
+template <typename T, int DF, int NK>
+__global__ void __launch_bounds__(256) k_xattn_fwd_few(Args<T> a) {
+    typedef Ty<T> Y;
+    typedef FewKeys<T, DF, NK> F;
+    typedef typename Y::frag frag;
+    typedef typename Y::half half;
+    constexpr int DT = F::DT, PITCH = F::PITCH;
+    __shared__ __attribute__((aligned(16))) char lds[2 * NK * F::TILE];
+    const int wi = work_item(a.blocks);
+    if (wi >= a.blocks) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int split = wi % a.nsplit, pair = wi / a.nsplit, b = pair / a.Hkv, hk = pair % a.Hkv;
+    const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
+    const unsigned on = F::live(a, a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr, len, lane);
+    const T* qb = a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh;
+    const int first = split * a.tiles_split, last = min(first + a.tiles_split, (a.M + 15) / 16);
+    frag nxt[DF];
+    load_rows<T, DF>(qb, a.q_st, a.q_sh, (first + wave) * 16 + li, a.M, a.G, a.D, g, nxt);
+    F::stage(lds, a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh, a.k_st, on, a.Tk, a.D);
+    F::stage(lds + NK * F::TILE, a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh, a.v_st, on, a.Tk, a.D);
+    __syncthreads();
+    frag k[NK][DF];
+    half vt[NK][DT];
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+#pragma unroll
+        for (int f = 0; f < DF; ++f) k[n][f] = frag_at<T>(lds, PITCH, n * 16 + li, f, g);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vt[n][d] = Y::read_t(lds + NK * F::TILE, PITCH, n * 16 + g * 4, d * 16, li);
+    }
+    const float scale2 = a.scale * LOG2E;
+    for (int tile = first + wave; tile < last; tile += 4) {
+        frag q[DF];
+#pragma unroll
+        for (int f = 0; f < DF; ++f) q[f] = nxt[f];
+        load_rows<T, DF>(qb, a.q_st, a.q_sh, (tile + 4) * 16 + li, a.M, a.G, a.D, g, nxt);
+        f32x4 s[NK];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+            s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int f = 0; f < DF; ++f) s[n] = Y::mma(k[n][f], q[f], s[n]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[n][r] = (on >> (n * 16 + g * 4 + r)) & 1 ? s[n][r] * scale2 : -INFINITY;
+                top = fmaxf(top, s[n][r]);
+            }
+        }
+        top = groups_max(top);
+        const float at = top == -INFINITY ? 0.f : top;
+        half hi[NK], lo[NK];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - at);
+                sum += s[n][r];
+            }
+            hi[n] = Y::pack(s[n]);
+            lo[n] = Y::rest(s[n], hi[n]);
+        }
+        sum = groups_sum(sum);
+        const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+        const int m = tile * 16 + li;
+        const size_t at_row = row_at(a, b, hk, min(m, a.M - 1));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < NK; ++n) o = Y::mma_parts(vt[n][d], hi[n], lo[n], o);
+            const int col = d * 16 + g * 4;
+            if (m < a.M && col < a.D) store_out(a, at_row + col, o * inv);
+        }
+        if (g == 0 && m < a.M && a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * LN2;
+    }
+}
+
+template <typename T, int DF, int NK>
+__global__ void __launch_bounds__(256) k_xattn_bwd_few(Args<T> a) {
+    typedef Ty<T> Y;
+    typedef FewKeys<T, DF, NK> F;
+    typedef typename Y::frag frag;
+    typedef typename Y::half half;
+    constexpr int DT = F::DT, PITCH = F::PITCH, DP = F::DP, OP = DP + 4;
+    constexpr int PIECES = Y::PARTS ? 2 : 1, SP = sizeof(T) == 4 ? 80 : 40, DS = NK * PIECES * 16 * SP;
+    constexpr int WAVE = 2 * F::TILE + DS, KEYS = 2 * NK * F::TILE, JOIN = 4 * 16 * OP * 4;
+    constexpr int LDS = KEYS > 4 * WAVE ? KEYS : 4 * WAVE;
+    __shared__ __attribute__((aligned(16))) char lds[LDS > JOIN ? LDS : JOIN];
+    const int wi = work_item(a.blocks);
+    if (wi >= a.blocks) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int split = wi % a.nsplit, pair = wi / a.nsplit, b = pair / a.Hkv, hk = pair % a.Hkv;
+    const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
+    const unsigned on = F::live(a, a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr, len, lane);
+    const T* qb = a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh;
+    const size_t out0 = row_at(a, b, hk, 0);
+    const T* rest_from = a.rest ? a.rest : a.o;              // (without a rest the outputs again, not used)
+    const int first = split * a.tiles_split, last = min(first + a.tiles_split, (a.M + 15) / 16);
+    const float scale2 = a.scale * LOG2E;
+
+    struct { frag q[DF], d_o[DF], o[DF], rest[DF]; float lse; } nxt;
+    auto fetch = [&](int tile) {
+        const int m = tile * 16 + li;
+        load_rows<T, DF>(qb, a.q_st, a.q_sh, m, a.M, a.G, a.D, g, nxt.q);
+        load_rows<T, DF>(a.dout + out0, (long)a.H * a.D, a.D, m, a.M, a.G, a.D, g, nxt.d_o);
+        load_rows<T, DF>(a.o + out0, (long)a.H * a.D, a.D, m, a.M, a.G, a.D, g, nxt.o);
+        if constexpr (Y::PARTS) load_rows<T, DF>(rest_from + out0, (long)a.H * a.D, a.D, m, a.M, a.G, a.D, g, nxt.rest);
+        nxt.lse = a.lse[stat_at(a, b, hk, min(m, a.M - 1))];
+    };
+    fetch(first + wave);
+    F::stage(lds, a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh, a.k_st, on, a.Tk, a.D);
+    F::stage(lds + NK * F::TILE, a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh, a.v_st, on, a.Tk, a.D);
+    __syncthreads();
+    frag k[NK][DF], v[NK][DF];
+    half kt[NK][DT];
+    f32x4 dk[NK][DT], dv[NK][DT];
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+#pragma unroll
+        for (int f = 0; f < DF; ++f) {
+            k[n][f] = frag_at<T>(lds, PITCH, n * 16 + li, f, g);
+            v[n][f] = frag_at<T>(lds + NK * F::TILE, PITCH, n * 16 + li, f, g);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            kt[n][d] = Y::read_t(lds, PITCH, n * 16 + g * 4, d * 16, li);
+            dk[n][d] = dv[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    __syncthreads();
+    char *lq = lds + wave * WAVE, *ldo = lq + F::TILE, *my_ds = ldo + F::TILE;
+
+    for (int tile = first + wave; tile < last; tile += 4) {
+        const int m = tile * 16 + li;
+        frag q[DF], d_o[DF];
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int f = 0; f < DF; ++f) {
+            q[f] = nxt.q[f];
+            d_o[f] = nxt.d_o[f];
+            s0 += Y::dot(d_o[f], nxt.o[f]);
+            if constexpr (Y::PARTS) s1 += Y::dot(d_o[f], nxt.rest[f]);
+        }
+        s0 = groups_sum(a.rest ? s0 + s1 : s0);
+        const float l = m < a.M ? nxt.lse * LOG2E : INFINITY;
+        fetch(tile + 4);
+        wave_lds_order();
+#pragma unroll
+        for (int f = 0; f < DF; ++f) {
+            *reinterpret_cast<frag*>(lq + li * PITCH + f * 64 + g * 16) = q[f];
+            *reinterpret_cast<frag*>(ldo + li * PITCH + f * 64 + g * 16) = d_o[f];
+        }
+        float lse[4], delta[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            delta[r] = __shfl(s0, g * 4 + r, 64);
+            lse[r] = __shfl(l, g * 4 + r, 64);
+        }
+        half p[NK], p_lo[NK], ds[NK], ds_lo[NK];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+            f32x4 s = {0.f, 0.f, 0.f, 0.f}, dp = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int f = 0; f < DF; ++f) {
+                s = Y::mma(q[f], k[n][f], s);
+                dp = Y::mma(d_o[f], v[n][f], dp);
+            }
+            const bool live = (on >> (n * 16 + li)) & 1;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[r] = live ? __builtin_amdgcn_exp2f(s[r] * scale2 - lse[r]) : 0.f;
+                dp[r] = live ? s[r] * (dp[r] - delta[r]) * a.scale : 0.f;
+            }
+            p[n] = Y::pack(s);
+            ds[n] = Y::pack(dp);
+            p_lo[n] = Y::rest(s, p[n]);
+            ds_lo[n] = Y::rest(dp, ds[n]);
+            *reinterpret_cast<half*>(my_ds + (n * 16 + li) * SP + g * (int)sizeof(half)) = ds[n];
+            if constexpr (Y::PARTS) *reinterpret_cast<half*>(my_ds + ((NK + n) * 16 + li) * SP + g * (int)sizeof(half)) = ds_lo[n];
+        }
+        wave_lds_order();
+        half dst[NK], dst_lo[NK];
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+            dst[n] = Y::read_t(my_ds, SP, n * 16 + g * 4, 0, li);
+            dst_lo[n] = Y::PARTS ? Y::read_t(my_ds, SP, (NK + n) * 16 + g * 4, 0, li) : dst[n];
+        }
+        const size_t at_row = row_at(a, b, hk, min(m, a.M - 1));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const half do_t = Y::read_t(ldo, PITCH, g * 4, d * 16, li), q_t = Y::read_t(lq, PITCH, g * 4, d * 16, li);
+            f32x4 dq = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                dv[n][d] = Y::mma_parts(do_t, p[n], p_lo[n], dv[n][d]);
+                dk[n][d] = Y::mma_parts(q_t, ds[n], ds_lo[n], dk[n][d]);
+                dq = Y::mma_parts(kt[n][d], dst[n], dst_lo[n], dq);
+            }
+            const int col = d * 16 + g * 4;
+            if (m < a.M && col < a.D) store4(a.dq + at_row + col, dq);
+        }
+    }
+
+    // the waves' sums joined; they leave, or go to the row range's slab: [range][pair][dk | dv][key][D]
+    float* jo = reinterpret_cast<float*>(lds);
+    const size_t slab = (size_t)2 * a.Tk * a.D, pairs = (size_t)a.B * a.Hkv;
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                *reinterpret_cast<f32x4*>(jo + (wave * 16 + li) * OP + d * 16 + g * 4) = which ? dv[n][d] : dk[n][d];
+            __syncthreads();
+            for (int c = threadIdx.x; c < 16 * (DP / 4); c += 256) {
+                const int r = c / (DP / 4), col = (c % (DP / 4)) * 4, key = n * 16 + r;
+                if (key >= a.Tk || col >= a.D) continue;
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x += *reinterpret_cast<const f32x4*>(jo + (i * 16 + r) * OP + col);
+                if (a.nsplit == 1) store4((which ? a.dv : a.dk) + (((size_t)b * a.Tk + key) * a.Hkv + hk) * a.D + col, x);
+                else *reinterpret_cast<f32x4*>(a.ws + (split * pairs + pair) * slab + ((size_t)which * a.Tk + key) * a.D + col) = x;
+            }
+        }
+}
+
+// the row ranges of dk and dv summed in range order
+template <typename T>
+__global__ void __launch_bounds__(256) k_xattn_few_join(Args<T> a) {
+    const int chunks = a.D / 4;
+    const size_t pairs = (size_t)a.B * a.Hkv, per = (size_t)2 * a.Tk * chunks, id = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= pairs * per) return;
+    const size_t pair = id / per;
+    const int in = (int)(id % per), col = (in % chunks) * 4, kk = in / chunks, which = kk / a.Tk, key = kk % a.Tk;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) x += *reinterpret_cast<const f32x4*>(a.ws + ((s * pairs + pair) * 2 * a.Tk + kk) * a.D + col);
+    store4((which ? a.dv : a.dk) + ((((pair / a.Hkv) * a.Tk + key) * a.Hkv) + pair % a.Hkv) * a.D + col, x);
+}
+
 // ---- many rows and many keys ------------------------------------------------------------------
 // Beyond 64 rows and 256 keys the matrix cores are the bound (14 M Tk / (M + Tk) flops per byte and 16-bit element, against
 // 230 that the card does per byte it reads), and what feeds them is LDS: a wave that reads a 16 x 16 key fragment once for
@@ -1433,11 +1698,24 @@ int key_splits(long items, int Tk, int dtype, bool tiled) {
 }
 bool one_pass(long M) { return M <= 32; }                    // the backward that keeps all rows of a pair on the chip
 bool tiled(long M, int Tk, int dtype) { return dtype == VQA_BF16 && M > 64 && Tk > 256; }        // k_xattn_*_tile
+bool few(long M, int Tk) { return Tk <= 32 && M > 32; }      // k_xattn_*_few
+// Row ranges of the few-keys kernels: two workgroups to a CU, of at least two row tiles per wave, at most 64 slabs
+int row_splits(long pairs, long M) {
+    const long tiles = (M + 15) / 16;
+    long n = (512 + pairs - 1) / pairs;
+    if (n > tiles / 8) n = tiles / 8;
+    if (n > 64) n = 64;
+    if (n < 1) n = 1;
+    const long per = (tiles + n - 1) / n;
+    return (int)((tiles + per - 1) / per);
+}
 // Waves of a tiled workgroup: eight share a key tile; four for so few rows that they take no more
 int tile_waves(long M) { return M <= 128 ? 4 : 8; }
 
 int fwd_splits(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
-    const long M = (long)Tq * (H / Hkv), mt = row_tiles(M, D, dtype), rows = tiled(M, Tk, dtype) ? 32 * tile_waves(M) : 16 * mt;
+    const long M = (long)Tq * (H / Hkv);
+    if (few(M, Tk)) return 1;                                // (its row ranges join nothing)
+    const long mt = row_tiles(M, D, dtype), rows = tiled(M, Tk, dtype) ? 32 * tile_waves(M) : 16 * mt;
     return key_splits((long)B * Hkv * ((M + rows - 1) / rows), Tk, dtype, tiled(M, Tk, dtype));
 }
 int bwd_splits(int B, int Tq, int Tk, int H, int Hkv, int dtype) { return key_splits((long)B * Hkv, Tk, dtype, false); }
@@ -1523,10 +1801,23 @@ Args<T> args_of(const VqaAttnView& q, const VqaAttnView& k, const VqaAttnView& v
         default: { constexpr int DF = 4; call; break; }                                        \
     }
 
+template <typename T> void few_plan(Args<T>& a) {
+    a.nsplit = row_splits((long)a.B * a.Hkv, a.M);
+    const int tiles = (a.M + 15) / 16;
+    a.tiles_split = (tiles + a.nsplit - 1) / a.nsplit;
+    a.blocks = a.B * a.Hkv * a.nsplit;
+}
+
 template <typename T>
 int fwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
     a.nsplit = nsplit;
-    bool done = false;
+    bool done = few(a.M, a.Tk);
+    if (done) {
+        few_plan(a);
+        const int grid = 8 * ((a.blocks + 7) / 8);
+        if (a.Tk <= 16) BY_WIDTH(T, a.D, (k_xattn_fwd_few<T, DF, 1><<<grid, 256, 0, stream>>>(a)));
+        else BY_WIDTH(T, a.D, (k_xattn_fwd_few<T, DF, 2><<<grid, 256, 0, stream>>>(a)));
+    }
     if constexpr (sizeof(T) == 2) {
         if (tiled(a.M, a.Tk, dtype)) {
             const int nw = tile_waves(a.M), tiles = (a.Tk + 63) / 64;
@@ -1568,6 +1859,17 @@ int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
         if (rc || nsplit == 1) return rc;
         const size_t n = (size_t)a.B * a.Hkv * a.M * (a.D / 4);
         k_xattn_dq_join<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a);
+        return vqa_check_launch("vqa_cross_attn_bwd (join)");
+    }
+    if (few(a.M, a.Tk)) {
+        few_plan(a);
+        const int grid = 8 * ((a.blocks + 7) / 8);
+        if (a.Tk <= 16) BY_WIDTH(T, a.D, (k_xattn_bwd_few<T, DF, 1><<<grid, 256, 0, stream>>>(a)));
+        else BY_WIDTH(T, a.D, (k_xattn_bwd_few<T, DF, 2><<<grid, 256, 0, stream>>>(a)));
+        int rc = vqa_check_launch("vqa_cross_attn_bwd");
+        if (rc || a.nsplit == 1) return rc;
+        const size_t n = (size_t)a.B * a.Hkv * 2 * a.Tk * (a.D / 4);
+        k_xattn_few_join<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a);
         return vqa_check_launch("vqa_cross_attn_bwd (join)");
     }
     const size_t rows = (size_t)a.B * a.Tq * a.H;
@@ -1615,7 +1917,12 @@ size_t vqa_cross_attn_fwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv
 }
 size_t vqa_cross_attn_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
     if (!sizes_ok(B, Tq, Tk, H, Hkv, D, dtype)) return 0;
-    if (!one_pass((long)Tq * (H / Hkv))) return (size_t)B * Tq * H;
+    const long M = (long)Tq * (H / Hkv);
+    if (few(M, Tk)) {
+        const int s = row_splits((long)B * Hkv, M);
+        return s > 1 ? (size_t)s * B * Hkv * 2 * Tk * D : 0;
+    }
+    if (!one_pass(M)) return (size_t)B * Tq * H;
     const int n = bwd_splits(B, Tq, Tk, H, Hkv, dtype);
     return n > 1 ? (size_t)n * B * Tq * H * D : 0;
 }
@@ -1644,7 +1951,8 @@ int vqa_cross_attn_bwd(const void* d_o, const VqaAttnView* q, const VqaAttnView*
     const int n = bwd_splits(B, Tq, Tk, H, Hkv, dtype);
     VQA_REQUIRE(d_o && o && lse && dq && dk && dv && aligned16(d_o) && aligned16(o) && aligned16(o_rest) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                 "vqa_cross_attn_bwd: d_o, o, lse, dq, dk, dv are needed, 16-byte aligned");
-    VQA_REQUIRE(aligned16(workspace) && (workspace || (n == 1 && one_pass((long)Tq * (H / Hkv)))), "vqa_cross_attn_bwd: this size needs the workspace");
+    VQA_REQUIRE(aligned16(workspace) && (workspace || vqa_cross_attn_bwd_workspace_floats(B, Tq, Tk, H, Hkv, D, dtype) == 0),
+                "vqa_cross_attn_bwd: this size needs the workspace");
     if (dtype == VQA_BF16) {
         Args<bf16_t> a = args_of<bf16_t>(*q, *k, *v, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D);
         a.dout = (const bf16_t*)d_o; a.o = (bf16_t*)o; a.rest = (bf16_t*)o_rest; a.lse = (float*)lse;

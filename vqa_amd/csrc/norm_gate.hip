@@ -172,7 +172,7 @@ struct Plan { int group, ngroups, sub, units, blocks; bool shared; };
 
 // rows a workgroup walks over: enough to make its slab (12 D bytes) small beside its rows, few enough to fill the chip
 Plan plan_of(long rows, int D, bool has_gate, long rows_per_gate) {
-    const Team t = team_of(D, rows);
+    const Team t = team_of(D, has_gate && rows_per_gate > 1 ? rows_per_gate : rows);
     const long waves = (long)t.lanes * t.teams / 64 > 0 ? (long)t.lanes * t.teams / 64 : 1;
     const long want = 256 * (12 / waves > 0 ? 12 / waves : 1);           // workgroups: 256 CUs, up to 12 waves on each
     long per = (rows + want - 1) / want;                                 // rows per workgroup
