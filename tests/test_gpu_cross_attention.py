@@ -133,6 +133,17 @@ def test_long_and_many(dtype):
         _check(q, k, v, do, kv_len=torch.full((B,), Tk // 3, device='cuda', dtype=torch.int32))
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('B,Tq,Tk,H,Hkv,D', [(1, 41, 1500, 8, 1, 72), (1, 35, 600, 1, 1, 64), (1, 301, 70, 3, 1, 40), (3, 37, 777, 5, 5, 128),
+                                             (1, 700, 300, 2, 1, 104), (1, 19, 31, 2, 1, 24)])
+def test_few_workgroups_split_keys_and_rows(B, Tq, Tk, H, Hkv, D, dtype):
+    """dq summed over ranges of keys, dk and dv over ranges of rows, where the pairs alone leave the chip empty."""
+    q, k, v, do = _inputs(B, Tq, Tk, H, Hkv, D, dtype, Tq)
+    _check(q, k, v, do)
+    mask = torch.rand(B, Tk, device='cuda', generator=torch.Generator(device='cuda').manual_seed(1)) < 0.7
+    _check(q, k, v, do, kv_len=torch.full((B,), Tk // 3, device='cuda', dtype=torch.int32), mask=mask)
+
+
 def test_strides_scale_and_sharp_scores():
     q, k, v, do = _inputs(2, 6, 37, 4, 2, 32, torch.bfloat16, 1, fused=False)
     want = _check(q, k, v, do, scale=0.3)

@@ -514,6 +514,18 @@ __global__ void __launch_bounds__(256) k_xattn_delta(Args<T> a, float* delta) {
     }
 }
 
+// four values of dq: out, or to the key range's slab
+template <typename T> __device__ __forceinline__ void leave_dq(const Args<T>& a, int split, int pair, int b, int hk, int m, int col, f32x4 x) {
+    if (a.nsplit == 1) store4(a.dq + row_at(a, b, hk, m) + col, x);
+    else *reinterpret_cast<f32x4*>(a.ws + (((size_t)split * a.B * a.Hkv + pair) * a.M + m) * a.D + col) = x;
+}
+// four values of dk (which 0) or dv (1): out, or to the row range's slab [range][pair][dk | dv][key][D]
+template <typename T> __device__ __forceinline__ void leave_dkv(const Args<T>& a, int split, int pair, int which, int key, int col, f32x4 x) {
+    const int b = pair / a.Hkv, hk = pair % a.Hkv;
+    if (a.nsplit == 1) store4((which ? a.dv : a.dk) + (((size_t)b * a.Tk + key) * a.Hkv + hk) * a.D + col, x);
+    else *reinterpret_cast<f32x4*>(a.ws + (((size_t)split * a.B * a.Hkv + pair) * 2 * a.Tk + (size_t)which * a.Tk + key) * a.D + col) = x;
+}
+
 // Rows of a pair all on the chip (M <= 16 MT): ONE pass over the keys for all three gradients.  A tile's values pass
 // through the wave's LDS for dP = dO V^T, then its keys for S = Q K^T (result tiles of 16 rows x 16 keys); P and
 // dS = scale P (dP - delta) from them are the B operands of dV^T = dO^T P and dK^T = Q^T dS; dS^T, through 16 x 16 pieces of
@@ -713,7 +725,6 @@ __global__ void __launch_bounds__(256) k_xattn_bwd(Args<T> a) {
     }
 
     float* jo = reinterpret_cast<float*>(lds);
-    const size_t rows = (size_t)a.B * a.Hkv * a.M;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         __syncthreads();
@@ -727,8 +738,7 @@ __global__ void __launch_bounds__(256) k_xattn_bwd(Args<T> a) {
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < W; ++i) x += *reinterpret_cast<const f32x4*>(jo + ((wave - w0 + i) * 16 + r) * OP + col);
-            if (a.nsplit == 1) store4(a.dq + row_at(a, b, hk, m) + col, x);
-            else *reinterpret_cast<f32x4*>(a.ws + ((size_t)split * rows + (size_t)pair * a.M + m) * a.D + col) = x;
+            leave_dq(a, split, pair, b, hk, m, col, x);
         }
     }
 }
@@ -747,22 +757,24 @@ __global__ void __launch_bounds__(256) k_xattn_dq_join(Args<T> a) {
 }
 
 // More rows than fit: the rows' side (dq) as the forward does it, rows in registers, key tiles streamed ...
-template <typename T, int DF, int MT>
+template <typename T, int DF, int MT, int W>
 __global__ void __launch_bounds__(256) k_xattn_bwd_q(Args<T> a) {
     typedef Ty<T> Y;
     typedef typename Y::frag frag;
     constexpr int DP = DF * Y::KC, DT = DP / 16, PITCH = DP * (int)sizeof(T) + Y::PAD, OP = DP + 4;
     constexpr int TILE = Y::KC * PITCH, JOIN = 4 * 16 * OP * 4;
     __shared__ __attribute__((aligned(16))) char lds[8 * TILE > JOIN ? 8 * TILE : JOIN];
-    const int wi = work_item(a.blocks);
-    if (wi >= a.blocks) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int rb = wi % a.row_blocks, pair = wi / a.row_blocks, b = pair / a.Hkv, hk = pair % a.Hkv, m0 = rb * 16 * MT;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, w0 = wave % W;
+    const int wi_ = work_item(a.blocks) * (4 / W) + wave / W;
+    const bool idle = wi_ >= a.items;                        // an item past the last one: no keys, nothing stored
+    const int wi = idle ? 0 : wi_, M = idle ? 0 : a.M;
+    const int rb = wi % a.row_blocks, ps = wi / a.row_blocks, split = ps % a.nsplit, pair = ps / a.nsplit;
+    const int b = pair / a.Hkv, hk = pair % a.Hkv, m0 = rb * 16 * MT;
     const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
     const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
     const T* kb = a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh;
     const T* vb = a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh;
-    const int last = (len + Y::KC - 1) / Y::KC;
+    const int first = split * a.tiles_split, last = idle ? 0 : min(first + a.tiles_split, (len + Y::KC - 1) / Y::KC);
     char *lk = lds + wave * 2 * TILE, *lv = lk + TILE;
     const float scale2 = a.scale * LOG2E;
     const size_t out0 = row_at(a, b, hk, 0);
@@ -773,27 +785,27 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_q(Args<T> a) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int m = m0 + mt * 16 + li;
-        load_rows<T, DF>(a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh, a.q_st, a.q_sh, m, a.M, a.G, a.D, g, q[mt]);
-        load_rows<T, DF>(a.dout + out0, (long)a.H * a.D, a.D, m, a.M, a.G, a.D, g, d_o[mt]);
+        load_rows<T, DF>(a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh, a.q_st, a.q_sh, m, M, a.G, a.D, g, q[mt]);
+        load_rows<T, DF>(a.dout + out0, (long)a.H * a.D, a.D, m, M, a.G, a.D, g, d_o[mt]);
         const size_t at = stat_at(a, b, hk, min(m, a.M - 1));
         const float l = a.lse[at];
         delta[mt] = a.delta[at];
-        lse[mt] = m < a.M ? l * LOG2E : INFINITY;
+        lse[mt] = m < M ? l * LOG2E : INFINITY;
 #pragma unroll
         for (int d = 0; d < DT; ++d) dq[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     Spots<T, DT> sp;
     sp.init(lane, a.D, Y::KC);
     KeyTile<T, DF> nxt;
-    nxt.load(a, sp, mask, len, kb, vb, wave * Y::KC, li);
+    nxt.load(a, sp, mask, len, kb, vb, (first + w0) * Y::KC, li);
     if (a.D < DP) wave_clear(lk, 2 * TILE, lane);
-    for (int tile = wave; tile < last; tile += 4) {
+    for (int tile = first + w0; tile < last; tile += W) {
         wave_lds_order();
         const KeyBits<T> bits = nxt.bits(mask != nullptr, len, tile * Y::KC, li);
         nxt.put(nxt.k, sp, bits, lk, PITCH);
         nxt.put(nxt.v, sp, bits, lv, PITCH);
         wave_lds_order();
-        nxt.load(a, sp, mask, len, kb, vb, (tile + 4) * Y::KC, li);
+        nxt.load(a, sp, mask, len, kb, vb, (tile + W) * Y::KC, li);
         if (!(bits.b[0] | bits.b[Y::NS - 1])) continue;
         typename Y::half h[MT][Y::NS], lo[MT][Y::NS];
 #pragma unroll
@@ -840,13 +852,13 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_q(Args<T> a) {
         for (int d = 0; d < DT; ++d)
             *reinterpret_cast<f32x4*>(jo + (wave * 16 + li) * OP + d * 16 + g * 4) = dq[mt][d];
         __syncthreads();
-        for (int c = threadIdx.x; c < 16 * (DP / 4); c += 256) {
+        for (int c = threadIdx.x % (64 * W); c < 16 * (DP / 4); c += 64 * W) {
             const int r = c / (DP / 4), col = (c % (DP / 4)) * 4, m = m0 + mt * 16 + r;
-            if (m >= a.M || col >= a.D) continue;
+            if (m >= M || col >= a.D) continue;
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x += *reinterpret_cast<const f32x4*>(jo + (i * 16 + r) * OP + col);
-            store4(a.dq + row_at(a, b, hk, m) + col, x * a.scale);
+            for (int i = 0; i < W; ++i) x += *reinterpret_cast<const f32x4*>(jo + ((wave - w0 + i) * 16 + r) * OP + col);
+            leave_dq(a, split, pair, b, hk, m, col, x * a.scale);
         }
     }
 }
@@ -864,7 +876,8 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_kv(Args<T> a) {
     const int wi = work_item(a.blocks);
     if (wi >= a.blocks) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int kblocks = a.row_blocks, kbk = wi % kblocks, pair = wi / kblocks, b = pair / a.Hkv, hk = pair % a.Hkv;
+    const int kblocks = a.row_blocks, kbk = wi % kblocks, ps = wi / kblocks, split = ps % a.nsplit, pair = ps / a.nsplit;
+    const int b = pair / a.Hkv, hk = pair % a.Hkv, m_first = split * a.tiles_split * Y::KC, m_last = min(m_first + a.tiles_split * Y::KC, a.M);
     const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
     const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
     const int key0 = (kbk * 4 + wave) * Y::KC;
@@ -885,7 +898,7 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_kv(Args<T> a) {
 
     const int wg_any = __syncthreads_or((int)(bits.b[0] | bits.b[Y::NS - 1]));
     if (wg_any) {
-        for (int m0 = 0; m0 < a.M; m0 += Y::KC) {
+        for (int m0 = m_first; m0 < m_last; m0 += Y::KC) {
             __syncthreads();
             // KC rows of q and dO, 16 bytes per thread at a time
             constexpr int CH = DP / Y::E;
@@ -956,20 +969,19 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_kv(Args<T> a) {
     for (int ns = 0; ns < Y::NS; ++ns) {
         const int key = key0 + ns * 16 + li;
         if (key >= a.Tk) continue;
-        const size_t at = (((size_t)b * a.Tk + key) * a.Hkv + hk) * a.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int c = d * 16 + g * 4;
             if (c < a.D) {
-                store4(a.dk + at + c, dk[ns][d] * a.scale);
-                store4(a.dv + at + c, dv[ns][d]);
+                leave_dkv(a, split, pair, 0, key, c, dk[ns][d] * a.scale);
+                leave_dkv(a, split, pair, 1, key, c, dv[ns][d]);
             }
         }
     }
 }
 
 // ---- few keys -------------------------------------------------------------------------------
-// At most 32 keys under more than 32 rows: the roles change.  The keys and values of a pair (NK tiles of 16) stay in every
+// At most 32 keys under more than 16 rows: the roles change.  The keys and values of a pair (NK tiles of 16) stay in every
 // wave's registers, the rows stream past, 16 at a time and each read once; scores of a row are complete at once, so the
 // softmax needs no second look; dq leaves with its rows, dk and dv are summed in registers over a wave's rows and joined
 // over waves and row ranges at the end.
@@ -1196,9 +1208,8 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_few(Args<T> a) {
         }
     }
 
-    // the waves' sums joined; they leave, or go to the row range's slab: [range][pair][dk | dv][key][D]
+    // the waves' sums joined
     float* jo = reinterpret_cast<float*>(lds);
-    const size_t slab = (size_t)2 * a.Tk * a.D, pairs = (size_t)a.B * a.Hkv;
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -1214,15 +1225,14 @@ __global__ void __launch_bounds__(256) k_xattn_bwd_few(Args<T> a) {
                 f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x += *reinterpret_cast<const f32x4*>(jo + (i * 16 + r) * OP + col);
-                if (a.nsplit == 1) store4((which ? a.dv : a.dk) + (((size_t)b * a.Tk + key) * a.Hkv + hk) * a.D + col, x);
-                else *reinterpret_cast<f32x4*>(a.ws + (split * pairs + pair) * slab + ((size_t)which * a.Tk + key) * a.D + col) = x;
+                leave_dkv(a, split, pair, which, key, col, x);
             }
         }
 }
 
 // the row ranges of dk and dv summed in range order
 template <typename T>
-__global__ void __launch_bounds__(256) k_xattn_few_join(Args<T> a) {
+__global__ void __launch_bounds__(256) k_xattn_dkv_join(Args<T> a) {
     const int chunks = a.D / 4;
     const size_t pairs = (size_t)a.B * a.Hkv, per = (size_t)2 * a.Tk * chunks, id = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= pairs * per) return;
@@ -1444,12 +1454,12 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
     const int wi = work_item(a.blocks);
     if (wi >= a.blocks) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int rb = wi % a.row_blocks, pair = wi / a.row_blocks, b = pair / a.Hkv, hk = pair % a.Hkv, m0 = (rb * NW + wave) * 16 * MT;
+    const int rb = wi % a.row_blocks, ps = wi / a.row_blocks, split = ps % a.nsplit, pair = ps / a.nsplit, b = pair / a.Hkv, hk = pair % a.Hkv, m0 = (rb * NW + wave) * 16 * MT;
     const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
     const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
     const bf16_t* kb = a.k + (size_t)b * a.k_sb + (size_t)hk * a.k_sh;
     const bf16_t* vb = a.v + (size_t)b * a.v_sb + (size_t)hk * a.v_sh;
-    const int last = (len + 63) / 64;
+    const int first = split * a.tiles_split, last = min(first + a.tiles_split, (len + 63) / 64);
     const size_t out0 = row_at(a, b, hk, 0);
 
     bf16x8_t q[MT][DF], d_o[MT][DF];
@@ -1477,7 +1487,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
             nxt.y[i] = vw.load((nxt.row(i) * (unsigned)a.v_st + nxt.col(i)) * 2u);
         }
     };
-    load(0);
+    load(first);
     f32x4 dq[MT][DT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -1485,13 +1495,13 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
         for (int d = 0; d < DT; ++d) dq[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float scale2 = a.scale * LOG2E;
     if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
-    unsigned long long on = live.bits(mask != nullptr, len, 0, lane);
+    unsigned long long on = live.bits(mask != nullptr, len, first * 64, lane);
     nxt.put(lds, lds + Tile::TILE, on);
-    load(1);
+    load(first + 1);
     __syncthreads();
 
     int cur = 0;
-    for (int tile = 0; tile < last; ++tile) {
+    for (int tile = first; tile < last; ++tile) {
         const char *lk = lds + cur * 2 * Tile::TILE, *lv = lk + Tile::TILE;
         const bool full = on == ~0ull;
 #pragma unroll
@@ -1543,7 +1553,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int col = d * 16 + g * 4;
-            if (col < a.D) store4(a.dq + row_at(a, b, hk, m) + col, dq[mt][d] * a.scale);
+            if (col < a.D) leave_dq(a, split, pair, b, hk, m, col, dq[mt][d] * a.scale);
         }
     }
 }
@@ -1561,7 +1571,8 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
     const int wi = work_item(a.blocks);
     if (wi >= a.blocks) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int kblocks = a.row_blocks, kbk = wi % kblocks, pair = wi / kblocks, b = pair / a.Hkv, hk = pair % a.Hkv;
+    const int kblocks = a.row_blocks, kbk = wi % kblocks, ps = wi / kblocks, split = ps % a.nsplit, pair = ps / a.nsplit;
+    const int b = pair / a.Hkv, hk = pair % a.Hkv, m_first = split * a.tiles_split * R, m_last = min(m_first + a.tiles_split * R, a.M);
     const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
     const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
     const int key0 = (kbk * NW + wave) * 32, block0 = kbk * NW * 32;
@@ -1600,13 +1611,13 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
             nxt.put(lds + buf * 2 * Tile::TILE, lds + buf * 2 * Tile::TILE + Tile::TILE, ~0ull);
             if (wave == 0 && lane < R) { l_lse[buf][lane] = n_lse; l_delta[buf][lane] = n_delta; }
         };
-        load(0);
+        load(m_first);
         if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
         put(0);
-        load(R);
+        load(m_first + R);
         __syncthreads();
         int cur = 0;
-        for (int m0 = 0; m0 < a.M; m0 += R) {
+        for (int m0 = m_first; m0 < m_last; m0 += R) {
             const char *lq = lds + cur * 2 * Tile::TILE, *ldo = lq + Tile::TILE;
 #pragma unroll
             for (int hf = 0; hf < R / 32; ++hf) {
@@ -1661,13 +1672,12 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
     for (int ns = 0; ns < 2; ++ns) {
         const int key = key0 + ns * 16 + li;
         if (key >= a.Tk) continue;
-        const size_t at = (((size_t)b * a.Tk + key) * a.Hkv + hk) * a.D;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int c = d * 16 + g * 4;
             if (c < a.D) {
-                store4(a.dk + at + c, dk[ns][d] * a.scale);
-                store4(a.dv + at + c, dv[ns][d]);
+                leave_dkv(a, split, pair, 0, key, c, dk[ns][d] * a.scale);
+                leave_dkv(a, split, pair, 1, key, c, dv[ns][d]);
             }
         }
     }
@@ -1698,7 +1708,9 @@ int key_splits(long items, int Tk, int dtype, bool tiled) {
 }
 bool one_pass(long M) { return M <= 32; }                    // the backward that keeps all rows of a pair on the chip
 bool tiled(long M, int Tk, int dtype) { return dtype == VQA_BF16 && M > 64 && Tk > 256; }        // k_xattn_*_tile
-bool few(long M, int Tk) { return Tk <= 32 && M > 32; }      // k_xattn_*_few
+// k_xattn_*_few (bf16, forward and backward: 256 x 20 rows on 20 x 8 heads 39 us, the streaming pair 48; 100 x 16 on 1 x 15
+// heads, two rows a head, 51 against 65; up to 16 rows both take one pass over as much)
+bool few(long M, int Tk) { return Tk <= 32 && M > 16; }
 // Row ranges of the few-keys kernels: two workgroups to a CU, of at least two row tiles per wave, at most 64 slabs
 int row_splits(long pairs, long M) {
     const long tiles = (M + 15) / 16;
@@ -1725,6 +1737,31 @@ int bwd_splits(int B, int Tq, int Tk, int H, int Hkv, int dtype) { return key_sp
 // 256 images x 15 heads: 66 against 61 us)
 int waves_of(const int items) { return items < 512 ? 4 : 2; }
 
+// The two-kernel backward: blocks, key ranges of the dq kernel, row ranges of the dk / dv kernel.  Ranges only where the
+// blocks alone leave CUs idle; row ranges of at least 4 tiles, at most 16 (slabs of dk and dv are as large as they are).
+// Forward and backward of bf16 2 x 509 rows on 2000 x 4 heads of 64: 75 us, 119 without ranges; fp32 2 x 200 on 200: 47, 56.
+size_t delta_floats(size_t rows) { return (rows + 3) / 4 * 4; }             // (the slabs behind it start at 16 bytes)
+struct TwoPlan { int row_blocks, key_splits, key_tiles, key_blocks, row_splits, row_tiles; };
+TwoPlan two_plan(int B, int Hkv, long M, int Tk, int D, int dtype) {
+    const bool tile = tiled(M, Tk, dtype);
+    const long pairs = (long)B * Hkv;
+    TwoPlan p;
+    const int rows = tile ? 32 * tile_waves(M) : 32, ktile = tile ? 64 : key_tile(dtype), ktiles = (Tk + ktile - 1) / ktile;
+    p.row_blocks = (int)((M + rows - 1) / rows);
+    p.key_splits = key_splits(pairs * p.row_blocks, Tk, dtype, tile);
+    p.key_tiles = (ktiles + p.key_splits - 1) / p.key_splits;
+    const int keys = tile ? 256 : 4 * key_tile(dtype), rtile = tile ? (D > 96 ? 32 : 64) : key_tile(dtype);
+    p.key_blocks = (Tk + keys - 1) / keys;
+    const long rtiles = (M + rtile - 1) / rtile, blocks = pairs * p.key_blocks;
+    long n = blocks >= 256 ? 1 : (512 + blocks - 1) / blocks;
+    if (n > rtiles / 4) n = rtiles / 4;
+    if (n > 16) n = 16;
+    if (n < 1) n = 1;
+    p.row_tiles = (int)((rtiles + n - 1) / n);
+    p.row_splits = (int)((rtiles + p.row_tiles - 1) / p.row_tiles);
+    return p;
+}
+
 template <typename T, int DF, int MT> void launch_fwd(const Args<T>& a, hipStream_t s) {
     const int grid = 8 * ((a.blocks + 7) / 8);
     if (waves_of(a.items) == 2) k_xattn_fwd<T, DF, MT, 2><<<grid, 256, 0, s>>>(a);
@@ -1745,15 +1782,10 @@ template <typename T, int DF> void launch_bwd(const Args<T>& a, hipStream_t s) {
         else k_xattn_bwd<T, DF, 1, 4><<<grid, 256, 0, s>>>(a);
     }
 }
-template <typename T, int DF> void launch_bwd_two(Args<T> a, hipStream_t s) {
-    constexpr int MT = 2;
-    const long pairs = (long)a.B * a.Hkv;
-    a.row_blocks = (a.M + 16 * MT - 1) / (16 * MT);
-    a.blocks = (int)(pairs * a.row_blocks);
-    k_xattn_bwd_q<T, DF, MT><<<8 * ((a.blocks + 7) / 8), 256, 0, s>>>(a);
-    a.row_blocks = (a.Tk + 4 * Ty<T>::KC - 1) / (4 * Ty<T>::KC);
-    a.blocks = (int)(pairs * a.row_blocks);
-    k_xattn_bwd_kv<T, DF><<<8 * ((a.blocks + 7) / 8), 256, 0, s>>>(a);
+template <typename T, int DF> void launch_bwd_q(const Args<T>& a, hipStream_t s) {
+    const int grid = 8 * ((a.blocks + 7) / 8);
+    if (waves_of(a.items) == 2) k_xattn_bwd_q<T, DF, 2, 2><<<grid, 256, 0, s>>>(a);
+    else k_xattn_bwd_q<T, DF, 2, 4><<<grid, 256, 0, s>>>(a);
 }
 
 // f<DF> with the number of fragments a row of D takes
@@ -1848,7 +1880,7 @@ int fwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
 
 template <typename T>
 int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
-    if (one_pass(a.M)) {
+    if (one_pass(a.M) && !few(a.M, a.Tk)) {
         a.nsplit = nsplit;
         const int tiles = (a.Tk + Ty<T>::KC - 1) / Ty<T>::KC;
         a.tiles_split = (tiles + nsplit - 1) / nsplit;
@@ -1869,29 +1901,52 @@ int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
         int rc = vqa_check_launch("vqa_cross_attn_bwd");
         if (rc || a.nsplit == 1) return rc;
         const size_t n = (size_t)a.B * a.Hkv * 2 * a.Tk * (a.D / 4);
-        k_xattn_few_join<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a);
+        k_xattn_dkv_join<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a);
         return vqa_check_launch("vqa_cross_attn_bwd (join)");
     }
     const size_t rows = (size_t)a.B * a.Tq * a.H;
-    k_xattn_delta<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(a, a.ws);
-    a.delta = a.ws;
+    const TwoPlan p = two_plan(a.B, a.Hkv, a.M, a.Tk, a.D, dtype);
+    float* const ws = a.ws;
+    k_xattn_delta<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(a, ws);
+    a.delta = ws;
+    // dq
+    a.row_blocks = p.row_blocks; a.nsplit = p.key_splits; a.tiles_split = p.key_tiles;
+    a.items = a.B * a.Hkv * a.row_blocks * a.nsplit;
+    float* const slabs = ws + delta_floats(rows);
+    a.ws = slabs;
+    const bool tile = tiled(a.M, a.Tk, dtype);
     if constexpr (sizeof(T) == 2) {
-        if (tiled(a.M, a.Tk, dtype)) {
-            const int nw = tile_waves(a.M);
-            a.row_blocks = (a.M + 32 * nw - 1) / (32 * nw);
-            a.blocks = a.B * a.Hkv * a.row_blocks;
-            int grid = 8 * ((a.blocks + 7) / 8);
-            if (nw == 8) { TILED(a.D, (k_xattn_bwd_q_tile<DF, 8><<<grid, 512, 0, stream>>>(a))) }
+        if (tile) {
+            a.blocks = a.items;
+            const int grid = 8 * ((a.blocks + 7) / 8);
+            if (tile_waves(a.M) == 8) { TILED(a.D, (k_xattn_bwd_q_tile<DF, 8><<<grid, 512, 0, stream>>>(a))) }
             else { TILED(a.D, (k_xattn_bwd_q_tile<DF, 4><<<grid, 256, 0, stream>>>(a))) }
-            a.row_blocks = (a.Tk + 255) / 256;
-            a.blocks = a.B * a.Hkv * a.row_blocks;
-            grid = 8 * ((a.blocks + 7) / 8);
-            TILED(a.D, (k_xattn_bwd_kv_tile<DF, 8><<<grid, 512, 0, stream>>>(a)))
-            return vqa_check_launch("vqa_cross_attn_bwd");
         }
     }
-    BY_WIDTH(T, a.D, (launch_bwd_two<T, DF>(a, stream)));
-    return vqa_check_launch("vqa_cross_attn_bwd");
+    if (!tile) {
+        a.blocks = waves_of(a.items) == 2 ? (a.items + 1) / 2 : a.items;
+        BY_WIDTH(T, a.D, (launch_bwd_q<T, DF>(a, stream)));
+    }
+    int rc = vqa_check_launch("vqa_cross_attn_bwd (dq)");
+    if (rc) return rc;
+    if (a.nsplit > 1) {
+        const size_t n = rows * (a.D / 4);
+        k_xattn_dq_join<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a);
+    }
+    // dk, dv
+    a.ws = slabs + (p.key_splits > 1 ? p.key_splits * rows * a.D : 0);
+    a.row_blocks = p.key_blocks; a.nsplit = p.row_splits; a.tiles_split = p.row_tiles;
+    a.blocks = a.B * a.Hkv * a.row_blocks * a.nsplit;
+    const int grid = 8 * ((a.blocks + 7) / 8);
+    if constexpr (sizeof(T) == 2) {
+        if (tile) { TILED(a.D, (k_xattn_bwd_kv_tile<DF, 8><<<grid, 512, 0, stream>>>(a))) }
+    }
+    if (!tile) BY_WIDTH(T, a.D, (k_xattn_bwd_kv<T, DF><<<grid, 256, 0, stream>>>(a)));
+    rc = vqa_check_launch("vqa_cross_attn_bwd (dk, dv)");
+    if (rc || a.nsplit == 1) return rc;
+    const size_t n = (size_t)a.B * a.Hkv * 2 * a.Tk * (a.D / 4);
+    k_xattn_dkv_join<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(a);
+    return vqa_check_launch("vqa_cross_attn_bwd (join)");
 }
 
 bool sizes_ok(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
@@ -1922,7 +1977,11 @@ size_t vqa_cross_attn_bwd_workspace_floats(int B, int Tq, int Tk, int H, int Hkv
         const int s = row_splits((long)B * Hkv, M);
         return s > 1 ? (size_t)s * B * Hkv * 2 * Tk * D : 0;
     }
-    if (!one_pass(M)) return (size_t)B * Tq * H;
+    if (!one_pass(M)) {
+        const TwoPlan p = two_plan(B, Hkv, M, Tk, D, dtype);
+        const size_t rows = (size_t)B * Tq * H;
+        return delta_floats(rows) + (p.key_splits > 1 ? p.key_splits * rows * D : 0) + (p.row_splits > 1 ? (size_t)p.row_splits * B * Hkv * 2 * Tk * D : 0);
+    }
     const int n = bwd_splits(B, Tq, Tk, H, Hkv, dtype);
     return n > 1 ? (size_t)n * B * Tq * H * D : 0;
 }
