@@ -266,6 +266,19 @@ __device__ __forceinline__ typename Ty<T>::frag frag_t(const char* lds, int pitc
     return Ty<T>::join(h);
 }
 
+// the same from a lane's own place (row g * 4 + li / 4, column 4 * (li % 4) of the tile's first 16 rows)
+__device__ __forceinline__ bf16x8_t frag_tr(const char* at, int pitch) {
+    typedef s16x4_t __attribute__((address_space(3))) * lds_p;
+    const s16x4_t h[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)at), __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + 16 * pitch))};
+    return Ty<bf16_t>::join(h);
+}
+
+// a value that all lanes hold, in a scalar register
+__device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+
+// keeps a uniform branch a branch: the compiler would select, element by element, on every pass
+__device__ __forceinline__ void rarely() { asm volatile(""); }
+
 template <typename T> __device__ __forceinline__ void store4(T* p, f32x4 v) {
     if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4*>(p) = v;
     else {
@@ -1269,14 +1282,18 @@ template <int DF, int NW, int R = 64> struct RowTile {
     static __device__ __forceinline__ Window window(const bf16_t* base, long st, long row0, int rows, int D) {
         return Window(base + (size_t)row0 * st, rows > 0 ? ((rows - 1) * (unsigned)st + D) * 2u : 0u);
     }
-    __device__ __forceinline__ void put(char* lx, char* ly, unsigned long long on) const {
-        const u32x4 z = {};
+    __device__ __forceinline__ void put(char* lx, char* ly, unsigned long long on) {
+        if (on != ~0ull) {
+            rarely();
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                if (!((on >> row(i)) & 1)) x[i] = y[i] = u32x4{};
+        }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const bool here = (on >> row(i)) & 1;
             const int at = row(i) * PITCH + col(i) * 2;
-            *reinterpret_cast<u32x4*>(lx + at) = here ? x[i] : z;
-            *reinterpret_cast<u32x4*>(ly + at) = here ? y[i] : z;
+            *reinterpret_cast<u32x4*>(lx + at) = x[i];
+            *reinterpret_cast<u32x4*>(ly + at) = y[i];
         }
     }
 };
@@ -1335,7 +1352,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
     };
     load(first);
     f32x4 o[MT][DT];
-    float mx[MT], sum[MT];                                   // mx: in units of the unscaled score
+    float mx[MT], sum[MT];                                   // mx: scaled, in powers of two
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         mx[mt] = -INFINITY;
@@ -1343,7 +1360,14 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const float scale2 = a.scale * LOG2E;
+    // scores stay unscaled, their maximum is found before the scale's product: that needs it positive (a negative one turns
+    // q's sign; of a zero, the least positive number makes the same weights)
+    const float scale2 = uniform(fmaxf(fabsf(a.scale) * LOG2E, 1e-37f));
+    if (a.scale < 0.f)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int f = 0; f < DF; ++f) q[mt][f] = -q[mt][f];
     if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
     unsigned long long on = live.bits(mask != nullptr, len, first * 64, lane), on_next = 0;
     nxt.put(lds, lds + Tile::TILE, on);
@@ -1366,19 +1390,24 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
             }
         }
         bf16x8_t p[MT][2];
-        const bool full = on == ~0ull;
+        if (on != ~0ull) {
+            rarely();
+#pragma unroll
+            for (int sub = 0; sub < 4; ++sub)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!((on >> (sub * 16 + g * 4 + r)) & 1))
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) s[mt][sub][r] = -INFINITY;
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             float top = -INFINITY;
 #pragma unroll
             for (int sub = 0; sub < 4; ++sub)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[mt][sub][r] *= scale2;
-                    if (!full) s[mt][sub][r] = (on >> (sub * 16 + g * 4 + r)) & 1 ? s[mt][sub][r] : -INFINITY;
-                    top = fmaxf(top, s[mt][sub][r]);
-                }
-            top = groups_max(top);
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[mt][sub][r]);
+            top = groups_max(top) * scale2;
             // the maximum follows only when a row's has grown by more than 2^8: until then p stays below 256, which
             // costs no accuracy, and the output need not be rescaled
             if (__any(top > mx[mt] + 8.f)) {
@@ -1394,7 +1423,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
             for (int sub = 0; sub < 4; ++sub) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[mt][sub][r] = __builtin_amdgcn_exp2f(s[mt][sub][r] - at);
+                    s[mt][sub][r] = __builtin_amdgcn_exp2f(s[mt][sub][r] * scale2 - at);
                     sum[mt] += s[mt][sub][r];
                 }
                 h[sub] = Y::pack(s[mt][sub]);
@@ -1472,7 +1501,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
         const size_t at = stat_at(a, b, hk, min(m, a.M - 1));
         const float l = a.lse[at];
         delta[mt] = a.delta[at];
-        lse[mt] = m < a.M ? l * LOG2E : INFINITY;
+        lse[mt] = m < a.M && l != -INFINITY ? l * LOG2E : INFINITY;        // (nothing attended: p = 0)
     }
     Tile nxt;
     Live64 live;
@@ -1493,7 +1522,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int d = 0; d < DT; ++d) dq[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float scale2 = a.scale * LOG2E;
+    const float scale2 = uniform(a.scale * LOG2E);
     if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
     unsigned long long on = live.bits(mask != nullptr, len, first * 64, lane);
     nxt.put(lds, lds + Tile::TILE, on);
@@ -1503,7 +1532,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
     int cur = 0;
     for (int tile = first; tile < last; ++tile) {
         const char *lk = lds + cur * 2 * Tile::TILE, *lv = lk + Tile::TILE;
-        const bool full = on == ~0ull;
+        if (on)                                              // (a tile that is masked throughout adds nothing)
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             Y::half h[MT][2];
@@ -1525,11 +1554,8 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float ds = __builtin_amdgcn_exp2f(s[mt][r] * scale2 - lse[mt]) * (dp[mt][r] - delta[mt]);
-                        if (!full) ds = (on >> (sub * 16 + g * 4 + r)) & 1 ? ds : 0.f;
-                        dp[mt][r] = ds;
-                    }
+                    for (int r = 0; r < 4; ++r)              // (a key that does not count is a row of zeros: its ds need only be finite)
+                        dp[mt][r] = __builtin_amdgcn_exp2f(fminf(s[mt][r] * scale2 - lse[mt], 1.f)) * (dp[mt][r] - delta[mt]);
                     h[mt][ns] = Y::pack(dp[mt]);
                 }
             }
@@ -1566,8 +1592,8 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
     constexpr int R = DF == 4 ? 32 : 64;                     // (at the widest rows a prefetch of 64 would not fit the registers)
     typedef RowTile<DF, NW, R> Tile;
     constexpr int DT = DF * 2, PITCH = Tile::PITCH;
-    __shared__ __attribute__((aligned(16))) char lds[4 * Tile::TILE];
-    __shared__ __attribute__((aligned(16))) float l_lse[2][R], l_delta[2][R];
+    // two tiles of q and dO rows, then the rows' lse and delta of each: [tile][lse | delta][row]
+    __shared__ __attribute__((aligned(16))) char lds[4 * Tile::TILE + 4 * R * 4];
     const int wi = work_item(a.blocks);
     if (wi >= a.blocks) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
@@ -1576,7 +1602,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
     const int len = a.kv_len ? max(0, min(a.kv_len[b], a.Tk)) : a.Tk;
     const uint8_t* mask = a.mask ? a.mask + (size_t)b * a.mask_sb : nullptr;
     const int key0 = (kbk * NW + wave) * 32, block0 = kbk * NW * 32;
-    const float scale2 = a.scale * LOG2E;
+    const float scale2 = uniform(a.scale * LOG2E);
     const bf16_t* qb = a.q + (size_t)b * a.q_sb + (size_t)hk * a.G * a.q_sh;
     const bf16_t* dob = a.dout + row_at(a, b, hk, 0);
 
@@ -1594,31 +1620,49 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
         Tile nxt;
         float n_lse, n_delta;
         nxt.init(a.D);
-        auto load = [&](int m0) {                            // rows past the last one repeat it; their p is zero
+        // the tile's rows as (token, head of the group): stepped from tile to tile, a division each would cost as much as
+        // the exponentials
+        const int dt = R / a.G, dh = R % a.G;
+        struct Row { int t, h; };
+        auto at_row = [&](int m) { Row r; r.t = m / a.G; r.h = m - r.t * a.G; return r; };
+        auto next = [&](Row& r) { r.t += dt; r.h += dh; if (r.h >= a.G) { r.h -= a.G; ++r.t; } };
+        Row rows[Tile::NI], stat = at_row(m_first + (lane & (R - 1)));
+#pragma unroll
+        for (int i = 0; i < Tile::NI; ++i) rows[i] = at_row(m_first + (int)nxt.row(i));
+        auto load = [&]() {                                  // rows past the last one read it again; their p is zero
 #pragma unroll
             for (int i = 0; i < Tile::NI; ++i) {
-                const int m = min(m0 + (int)nxt.row(i), a.M - 1), t = m / a.G, hh = m - t * a.G;
+                const int t = min(rows[i].t, a.Tq - 1), hh = rows[i].h;
                 nxt.x[i] = *reinterpret_cast<const u32x4*>(qb + (size_t)t * a.q_st + (size_t)hh * a.q_sh + nxt.col(i));
                 nxt.y[i] = *reinterpret_cast<const u32x4*>(dob + ((size_t)t * a.H + hh) * a.D + nxt.col(i));
+                next(rows[i]);
             }
-            const int m = m0 + (lane & (R - 1));
-            const size_t at = stat_at(a, b, hk, min(m, a.M - 1));
+            const size_t at = ((size_t)b * a.H + hk * a.G + stat.h) * a.Tq + min(stat.t, a.Tq - 1);
             const float l = a.lse[at];
             n_delta = a.delta[at];
-            n_lse = m < a.M ? l * LOG2E : INFINITY;
+            n_lse = stat.t < a.Tq ? l * LOG2E : INFINITY;
+            next(stat);
         };
         auto put = [&](int buf) {
             nxt.put(lds + buf * 2 * Tile::TILE, lds + buf * 2 * Tile::TILE + Tile::TILE, ~0ull);
-            if (wave == 0 && lane < R) { l_lse[buf][lane] = n_lse; l_delta[buf][lane] = n_delta; }
+            if (wave == 0 && lane < R) {
+                float* st = reinterpret_cast<float*>(lds + 4 * Tile::TILE) + buf * 2 * R + lane;
+                st[0] = n_lse;
+                st[R] = n_delta;
+            }
         };
-        load(m_first);
+        load();
         if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
         put(0);
-        load(m_first + R);
+        load();
         __syncthreads();
+        // a lane's places in a tile, as one number each (the compiler would keep their parts)
+        int at_frag = li * PITCH + g * 16, at_t = (g * 4 + (li >> 2)) * PITCH + (li & 3) * 8;
+        asm volatile("" : "+v"(at_frag), "+v"(at_t));
         int cur = 0;
         for (int m0 = m_first; m0 < m_last; m0 += R) {
-            const char *lq = lds + cur * 2 * Tile::TILE, *ldo = lq + Tile::TILE;
+            const char* lq = lds + cur * 2 * Tile::TILE;         // q rows; dO rows a TILE behind
+            const float* lst = reinterpret_cast<const float*>(lds + 4 * Tile::TILE) + cur * 2 * R;
 #pragma unroll
             for (int hf = 0; hf < R / 32; ++hf) {
                 Y::half p[2][2], ds[2][2];                   // [key tile][row tile]
@@ -1630,31 +1674,32 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
                     for (int ns = 0; ns < 2; ++ns) s[ns] = dp[ns] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int f = 0; f < DF; ++f) {
-                        const bf16x8_t qf = frag_at<bf16_t>(lq, PITCH, row + li, f, g), df = frag_at<bf16_t>(ldo, PITCH, row + li, f, g);
+                        const char* at = lq + at_frag + row * PITCH + f * 64;
+                        const bf16x8_t qf = *reinterpret_cast<const bf16x8_t*>(at), df = *reinterpret_cast<const bf16x8_t*>(at + Tile::TILE);
 #pragma unroll
                         for (int ns = 0; ns < 2; ++ns) {
                             s[ns] = Y::mma(qf, k[ns][f], s[ns]);
                             dp[ns] = Y::mma(df, v[ns][f], dp[ns]);
                         }
                     }
-                    const f32x4 ls = *reinterpret_cast<const f32x4*>(&l_lse[cur][row + g * 4]);
-                    const f32x4 de = *reinterpret_cast<const f32x4*>(&l_delta[cur][row + g * 4]);
+                    const f32x4 ls = *reinterpret_cast<const f32x4*>(lst + row + g * 4);
+                    const f32x4 de = *reinterpret_cast<const f32x4*>(lst + R + row + g * 4);
 #pragma unroll
                     for (int ns = 0; ns < 2; ++ns) {
-                        const bool on = (bits.b[ns] >> li) & 1;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            s[ns][r] = on ? __builtin_amdgcn_exp2f(s[ns][r] * scale2 - ls[r]) : 0.f;
+                        for (int r = 0; r < 4; ++r) {        // (a key that does not count: its own sums, dropped at the end)
+                            s[ns][r] = __builtin_amdgcn_exp2f(s[ns][r] * scale2 - ls[r]);
                             dp[ns][r] = s[ns][r] * (dp[ns][r] - de[r]);
                         }
                         p[ns][qs] = Y::pack(s[ns]);
                         ds[ns][qs] = Y::pack(dp[ns]);
+                        asm volatile("" : "+v"(p[ns][qs]), "+v"(ds[ns][qs]));
                     }
                 }
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const bf16x8_t dot_ = frag_t<bf16_t>(ldo + hf * 32 * PITCH, PITCH, d * 16, li, g);
-                    const bf16x8_t qt = frag_t<bf16_t>(lq + hf * 32 * PITCH, PITCH, d * 16, li, g);
+                    const char* at = lq + at_t + hf * 32 * PITCH + d * 32;
+                    const bf16x8_t qt = frag_tr(at, PITCH), dot_ = frag_tr(at + Tile::TILE, PITCH);
 #pragma unroll
                     for (int ns = 0; ns < 2; ++ns) {
                         dv[ns][d] = Y::mma(dot_, Y::join(p[ns]), dv[ns][d]);
@@ -1664,7 +1709,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
             }
             cur ^= 1;
             put(cur);
-            load(m0 + 2 * R);
+            load();
             __syncthreads();
         }
     }
@@ -1672,12 +1717,14 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
     for (int ns = 0; ns < 2; ++ns) {
         const int key = key0 + ns * 16 + li;
         if (key >= a.Tk) continue;
+        const bool on = (bits.b[ns] >> li) & 1;
+        const f32x4 z = {};
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int c = d * 16 + g * 4;
             if (c < a.D) {
-                leave_dkv(a, split, pair, 0, key, c, dk[ns][d] * a.scale);
-                leave_dkv(a, split, pair, 1, key, c, dv[ns][d]);
+                leave_dkv(a, split, pair, 0, key, c, on ? dk[ns][d] * a.scale : z);
+                leave_dkv(a, split, pair, 1, key, c, on ? dv[ns][d] : z);
             }
         }
     }
