@@ -51,7 +51,7 @@ def _bounds(q, k, v, do, o, lse, live, scale):
     dabs = (DO * O).abs().sum(-1, keepdim=True)
     ds = (p * (dp - delta)).abs() + p * (DO.abs() @ V.abs().transpose(2, 3).contiguous()) * 2.0 ** -8 + p * dabs
     pa = p
-    return (back(pa @ V.abs()), back(ds @ K.abs()) * scale, (ds.transpose(2, 3).contiguous() @ Q.abs()).transpose(1, 2) * scale,
+    return (back(pa @ V.abs()), back(ds @ K.abs()) * abs(scale), (ds.transpose(2, 3).contiguous() @ Q.abs()).transpose(1, 2) * abs(scale),
             (pa.transpose(2, 3).contiguous() @ DO.abs()).transpose(1, 2))
 
 
@@ -160,6 +160,20 @@ def test_strides_scale_and_sharp_scores():
     q, k, v, do = _inputs(1, 20, 300, 2, 2, 64, torch.float32, 2, fused=False)
     k[:, 271] = 6 * q[:, 3]
     _check(q, k, v, do)
+
+
+@pytest.mark.parametrize('shape', [(2, 7, 90, 2, 2, 64), (1, 40, 70, 4, 2, 64), (2, 90, 400, 2, 2, 64), (2, 40, 20, 3, 1, 64)])
+@pytest.mark.parametrize('scale', [0.6, -0.6, 0.0, -1e-3])
+def test_scores_far_below_zero_and_signs_of_the_scale(shape, scale):
+    """Scores near -115 (0.6), where a masked key's 0 would be exp(115) times more than any that counts; a scale that turns
+    them, and none.  |z| of 115 is good to 115 x 2^-21, below a bf16 half step's thirtieth."""
+    q, k, v, do = _inputs(*shape, torch.bfloat16, 9, fused=False)
+    q, k = (q * 0.05 + 1).bfloat16(), (k * 0.05 - 3).bfloat16()
+    B, Tk = shape[0], shape[2]
+    mask = torch.rand(B, Tk, device='cuda', generator=torch.Generator(device='cuda').manual_seed(2)) < 0.6
+    mask[0] = False
+    _check(q, k, v, do, scale=scale)
+    _check(q, k, v, do, kv_len=torch.full((B,), Tk - 5, device='cuda', dtype=torch.int32), mask=mask, scale=scale)
 
 
 def test_infinite_and_nan_operands_spread_as_in_the_formula():
