@@ -7,7 +7,12 @@
 // reads its 8 steps into registers and folds them, the waves' maps are chained through LDS, and every wave then walks its
 // steps again from its true starting state, out of registers, while the next block is on its way.  Only where the units of
 // all samples together make too few workgroups is time itself cut into chunks for different workgroups; the maps of the
-// chunks then take a pass over the gates of their own.
+// chunks then take a pass over the gates of their own (with an atomic-free chain between the passes).
+// Measured (bf16): 256 x 14 steps of 2400 units, ragged, 17 us forward and 31 backward; 1 x 16001 steps of 2048 units, cut
+// into 251 chunks, 50 (maps) + 57 us forward, 3.9 and 5.7 TB/s, and 80 + 129 us backward, 4.1 and 4.6 TB/s, where a large
+// copy reaches 5.1; 7 x 577 steps of 1200 units, fp32, 27 and 44 us.  At ten transcendental instructions a step and unit the
+// arithmetic takes about half of that.  Sixteen waves to a workgroup (half the blocks) made the backward spill, narrower
+// tiles of units with more shares of steps per wave gained nothing.
 #include "common.h"
 #include "vqa_hip.h"
 
@@ -169,24 +174,30 @@ __global__ void __launch_bounds__(MOST_WAVES * 64) k_scan_fwd(Args<T> a) {
 }
 
 // carry[k] for k = 1 .. nchunk - 1 (FORWARD: from c0 on; otherwise from dc_last back, carry[k] is what reaches the END of
-// chunk k).  A workgroup takes 32 (sample, unit) columns and cuts the chunks into 8 runs: every thread folds its run, the
-// runs are chained through LDS, then every thread walks its run again from its true start.
+// chunk k).  A workgroup takes 32 (sample, unit) columns and cuts the chunks into 32 runs: every thread folds its run, the
+// runs are chained through LDS, then every thread walks its run again from its true start.  Latency is all there is to
+// it: 32 runs (8 chunks each for 16001 steps, read at once) take 5.4 us, 8 runs of 32 chunks 9.0.
+constexpr int RUNS = 32;
 template <typename T, bool FORWARD>
-__global__ void __launch_bounds__(256) k_scan_chain(Args<T> a) {
-    __shared__ float sp[8][33], sa[8][33];
+__global__ void __launch_bounds__(RUNS * 32) k_scan_chain(Args<T> a) {
+    __shared__ float sp[RUNS][33], sa[RUNS][33];
     const int cx = threadIdx.x & 31, run = threadIdx.x >> 5;
     const long plane = (long)a.B * a.H, col = (long)blockIdx.x * 32 + cx;
     const bool on = col < plane;
     const int n = a.nchunk - 1;                              // maps applied: chunks 0 .. n-1, or n .. 1
-    const int per = (n + 7) / 8, lo = min(run * per, n), hi = min(lo + per, n);
+    const int per = (n + RUNS - 1) / RUNS, lo = min(run * per, n), hi = min(lo + per, n);
     auto at = [&](int s) { return (FORWARD ? s : a.nchunk - 1 - s) * plane + col; };
-    float P = 1.f, A = 0.f;
+    float p[8], q[8], P = 1.f, A = 0.f;
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (s0 + j < hi) { p[j] = a.prod[at(s0 + j)]; q[j] = a.add[at(s0 + j)]; }
+    };
+    const float* first = FORWARD ? a.c0 : a.dc_last;
+    float x = on && first ? first[col] : 0.f;
     if (on)
         for (int s0 = lo; s0 < hi; s0 += 8) {
-            float p[8], q[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (s0 + j < hi) { p[j] = a.prod[at(s0 + j)]; q[j] = a.add[at(s0 + j)]; }
+            fetch(s0);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (s0 + j < hi) { A = p[j] * A + q[j]; P *= p[j]; }
@@ -195,15 +206,10 @@ __global__ void __launch_bounds__(256) k_scan_chain(Args<T> a) {
     sa[run][cx] = A;
     __syncthreads();
     if (!on) return;
-    const float* first = FORWARD ? a.c0 : a.dc_last;
-    float x = first ? first[col] : 0.f;
     if (!FORWARD && run == 0) a.carry[(a.nchunk - 1) * plane + col] = x;
     for (int r = 0; r < run; ++r) x = sp[r][cx] * x + sa[r][cx];
     for (int s0 = lo; s0 < hi; s0 += 8) {
-        float p[8], q[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (s0 + j < hi) { p[j] = a.prod[at(s0 + j)]; q[j] = a.add[at(s0 + j)]; }
+        if (per > 8) fetch(s0);                              // (otherwise they are still there)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (s0 + j < hi) {
@@ -356,7 +362,7 @@ template <typename T> int fwd(Args<T> a, float* ws, int dtype, hipStream_t strea
     const size_t lds = (size_t)threads * 4 * Raw<T>::V * sizeof(float);
     if (a.nchunk > 1) {
         k_scan_fwd<T, true, false, true><<<dim3(grid.x, grid.y - 1), threads, lds, stream>>>(a);
-        k_scan_chain<T, true><<<(unsigned)(((long)a.B * a.H + 31) / 32), 256, 0, stream>>>(a);
+        k_scan_chain<T, true><<<(unsigned)(((long)a.B * a.H + 31) / 32), RUNS * 32, 0, stream>>>(a);
     }
     const bool one = a.chunk <= threads / 64 * SAVE;
     if (a.saved) {
@@ -374,7 +380,7 @@ template <typename T> int bwd(Args<T> a, float* ws, int dtype, hipStream_t strea
     const size_t lds = (size_t)threads * 4 * Raw<T>::V * sizeof(float);
     if (a.nchunk > 1) {
         k_scan_bwd<T, true, true><<<dim3(grid.x, grid.y - 1), threads, lds, stream>>>(a);
-        k_scan_chain<T, false><<<(unsigned)(((long)a.B * a.H + 31) / 32), 256, 0, stream>>>(a);
+        k_scan_chain<T, false><<<(unsigned)(((long)a.B * a.H + 31) / 32), RUNS * 32, 0, stream>>>(a);
     }
     if (a.chunk <= threads / 64 * SAVE) k_scan_bwd<T, false, true><<<grid, threads, lds, stream>>>(a);
     else k_scan_bwd<T, false, false><<<grid, threads, lds, stream>>>(a);

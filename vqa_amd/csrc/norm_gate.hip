@@ -7,7 +7,12 @@
 // registers, 8 columns per thread, from its one load to its one store: a TEAM of threads owns a row, as many as the row
 // has 16-byte (bf16) chunks, rounded up to a power of two inside a wave or to whole waves beyond; a workgroup of about
 // 256 threads holds several teams and walks over rows, so the fp32 per-column weights stay in registers too (read per
-// row they would be more L2 traffic than the row itself).
+// row they would be more L2 traffic than the row itself); the backward, which needs them beside five operands and three
+// running column sums, keeps them in LDS instead (in registers it spilled).  Column sums leave a workgroup as one slab row
+// and a second kernel adds the slabs in order.
+// Measured (a large copy reaches 5.1 TB/s): 100352 rows of 2048, bf16, a gate row per 196: forward 352 us (4.7 TB/s),
+// backward 517 + 15 us (4.8 TB/s); 3570 rows of 2400, fp32, a gate per row: 46 us (3.7 TB/s) and 66 + 5 us (4.1 TB/s);
+// 14 rows of 1200: 4.5 us.
 #include "common.h"
 #include "vqa_hip.h"
 
