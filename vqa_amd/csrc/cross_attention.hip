@@ -216,13 +216,14 @@ template <typename T, int NI> struct Spots {                 // lane's chunks: r
         const unsigned per = D / Ty<T>::E, inv = (65536 + per - 1) / per;      // c / per, exact for c < 1024, per <= 32
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const unsigned c = min((unsigned)(i * 64 + lane), per * rows - 1), r = (c * inv) >> 16;
-            rc[i] = (int)(r | (c - r * per) << 8);
+            const unsigned c = min((unsigned)(i * 64 + lane), per * rows - 1), r = __umul24(c, inv) >> 16;
+            rc[i] = (int)(r | (c - __umul24(r, per)) << 8);
         }
     }
     __device__ __forceinline__ unsigned row(int i) const { return rc[i] & 255; }
     __device__ __forceinline__ unsigned col(int i) const { return (rc[i] >> 8) * Ty<T>::E; }
-    __device__ __forceinline__ unsigned at(int i, unsigned st) const { return (row(i) * st + col(i)) * (unsigned)sizeof(T); }
+    // (strides are multiples of 8 below 2^25: a product of 24 bits, which takes a quarter of a full one's time)
+    __device__ __forceinline__ unsigned at(int i, unsigned st) const { return ((__umul24(row(i), st >> 3) << 3) + col(i)) * (unsigned)sizeof(T); }
 };
 template <typename T, int DF> struct KeyTile {
     typedef Ty<T> Y;
@@ -295,6 +296,10 @@ __device__ __forceinline__ bf16x8_t frag_tr(const char* at, int pitch) {
 // a value that all lanes hold, in a scalar register
 __device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
 
+// The forward finds a row's largest score before the scale's product (the exponential takes both in one instruction), which
+// needs a positive one: a negative scale turns q's sign, and of a zero the least positive number makes the same weights.
+__device__ __forceinline__ float positive_scale(float scale) { return uniform(fmaxf(fabsf(scale) * LOG2E, 1e-37f)); }
+
 // keeps a uniform branch a branch: the compiler would select, element by element, on every pass
 __device__ __forceinline__ void rarely() { asm volatile(""); }
 
@@ -320,10 +325,16 @@ template <typename T> __device__ __forceinline__ void store_out(const Args<T>& a
     }
 }
 
-// element offset of row m of pair (b, hk) in a (B, Tq, H, D) array
-template <typename T> __device__ __forceinline__ size_t row_at(const Args<T>& a, int b, int hk, int m) {
+// element offset of pair (b, hk) in a (B, Tq, H, D) array, and the place n of its row m there: n D further on
+template <typename T> __device__ __forceinline__ size_t pair_at(const Args<T>& a, int b, int hk) {
+    return ((size_t)b * a.Tq * a.H + hk * a.G) * a.D;
+}
+template <typename T> __device__ __forceinline__ int place_of(const Args<T>& a, int m) {
     const int t = m / a.G;
-    return (((size_t)b * a.Tq + t) * a.H + hk * a.G + (m - t * a.G)) * a.D;
+    return t * a.H + (m - t * a.G);
+}
+template <typename T> __device__ __forceinline__ size_t row_at(const Args<T>& a, int b, int hk, int m) {
+    return pair_at(a, b, hk) + (size_t)place_of(a, m) * a.D;
 }
 template <typename T> __device__ __forceinline__ size_t stat_at(const Args<T>& a, int b, int hk, int m) {
     const int t = m / a.G;
@@ -343,6 +354,7 @@ __global__ void __launch_bounds__(256, waves_fwd<T>(DF, MT)) k_xattn_fwd(Args<T>
     constexpr int TILE = Y::KC * PITCH, JOIN = 4 * 16 * OP * 4;
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE > JOIN ? 4 * TILE : JOIN];
     __shared__ float sm[4][16 * MT], sl[4][16 * MT];
+    __shared__ int places[4 / W][16 * MT];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, w0 = wave % W;
     const int wi_ = work_item(a.blocks) * (4 / W) + wave / W;
     const bool idle = wi_ >= a.items;                        // an item past the last one: no keys, nothing stored
@@ -373,7 +385,14 @@ __global__ void __launch_bounds__(256, waves_fwd<T>(DF, MT)) k_xattn_fwd(Args<T>
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const float scale2 = a.scale * LOG2E;
+    const float scale2 = positive_scale(a.scale);
+    if (a.scale < 0.f) {
+        rarely();
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int f = 0; f < DF; ++f) q[mt][f] = -q[mt][f];
+    }
     const bool spare = a.D <= DP - 16;                       // the last 16 columns are all padding
     if (a.D < DP) wave_clear(my, TILE, lane);
 
@@ -399,18 +418,25 @@ __global__ void __launch_bounds__(256, waves_fwd<T>(DF, MT)) k_xattn_fwd(Args<T>
         nxt.put(nxt.v, sp, bits, my, PITCH);
         wave_lds_order();
         nxt.load_v(a, sp, len, vb, (tile + W) * Y::KC);
-        frag p[MT], p_lo[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float top = mx[mt];
+        if ((bits.b[0] & bits.b[Y::NS - 1]) != 0xffffu) {
+            rarely();
 #pragma unroll
             for (int ns = 0; ns < Y::NS; ++ns)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[mt][ns][r] = (bits.b[ns] >> (g * 4 + r)) & 1 ? s[mt][ns][r] * scale2 : -INFINITY;
-                    top = fmaxf(top, s[mt][ns][r]);
-                }
-            top = groups_max(top);
+                for (int r = 0; r < 4; ++r)
+                    if (!((bits.b[ns] >> (g * 4 + r)) & 1))
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) s[mt][ns][r] = -INFINITY;
+        }
+        frag p[MT], p_lo[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int ns = 0; ns < Y::NS; ++ns)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[mt][ns][r]);
+            top = fmaxf(groups_max(top) * scale2, mx[mt]);
             const float at = top == -INFINITY ? 0.f : top;
             const float shrink = __builtin_amdgcn_exp2f(mx[mt] - at);
             mx[mt] = top;
@@ -420,7 +446,7 @@ __global__ void __launch_bounds__(256, waves_fwd<T>(DF, MT)) k_xattn_fwd(Args<T>
             for (int ns = 0; ns < Y::NS; ++ns) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[mt][ns][r] = __builtin_amdgcn_exp2f(s[mt][ns][r] - at);
+                    s[mt][ns][r] = __builtin_amdgcn_exp2f(s[mt][ns][r] * scale2 - at);
                     sum[mt] += s[mt][ns][r];
                 }
                 h[ns] = Y::pack(s[mt][ns]);
@@ -445,50 +471,56 @@ __global__ void __launch_bounds__(256, waves_fwd<T>(DF, MT)) k_xattn_fwd(Args<T>
         }
     }
 
-    // join the item's waves: row by row the common maximum, then the sums
-    const size_t rows = (size_t)a.B * a.Hkv * a.M;
-    const int w1 = wave - w0;                                // the item's first wave
+    // join the item's waves: one thread per row finds the common maximum, the sum and what each wave's output counts for
+    const size_t rows = (size_t)a.B * a.Hkv * a.M, row0 = (size_t)split * rows + (size_t)pair * a.M + m0;
+    const int w1 = wave - w0, it = threadIdx.x % (64 * W);   // the item's first wave; the thread in the item
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const float l = groups_sum(sum[mt]);
         if (g == 0) { sm[wave][mt * 16 + li] = mx[mt]; sl[wave][mt * 16 + li] = l; }
     }
+    __syncthreads();
+    if (it < 16 * MT) {
+        float top = sm[w1][it], l = 0.f, w[W];
+#pragma unroll
+        for (int i = 1; i < W; ++i) top = fmaxf(top, sm[w1 + i][it]);
+        const float at = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            w[i] = __builtin_amdgcn_exp2f(sm[w1 + i][it] - at);
+            l += w[i] * sl[w1 + i][it];
+        }
+        const float inv = a.nsplit > 1 ? 1.f : top == -INFINITY ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < W; ++i) sm[w1 + i][it] = w[i] * inv;
+        const int m = m0 + it;
+        places[wave / W][it] = place_of(a, m);
+        if (m < M) {
+            if (a.nsplit > 1) {
+                float* st = a.ws + ((size_t)a.nsplit * rows * a.D + (row0 + it) * 2);
+                st[0] = top;
+                st[1] = l;
+            } else if (a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(l)) * LN2;
+        }
+    }
     float* jo = reinterpret_cast<float*>(lds);
+    const size_t out0 = pair_at(a, b, hk);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        __syncthreads();
+        if (mt > 0) __syncthreads();
 #pragma unroll
         for (int d = 0; d < DT; ++d)
             *reinterpret_cast<f32x4*>(jo + (wave * 16 + li) * OP + d * 16 + g * 4) = o[mt][d];
         __syncthreads();
-        for (int c = threadIdx.x % (64 * W); c < 16 * (DP / 4); c += 64 * W) {
-            const int r = c / (DP / 4), col = (c % (DP / 4)) * 4, m = m0 + mt * 16 + r;
-            if (m >= M) continue;
-            float top = sm[w1][mt * 16 + r];
-#pragma unroll
-            for (int i = 1; i < W; ++i) top = fmaxf(top, sm[w1 + i][mt * 16 + r]);
-            const float at = top == -INFINITY ? 0.f : top;
-            float l = 0.f;
+#pragma unroll 2
+        for (int c = it; c < 16 * (DP / 4); c += 64 * W) {
+            const int r = c / (DP / 4), col = (c % (DP / 4)) * 4, row = mt * 16 + r;
+            if (m0 + row >= M || col >= a.D) continue;
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float w = __builtin_amdgcn_exp2f(sm[w1 + i][mt * 16 + r] - at);
-                l += w * sl[w1 + i][mt * 16 + r];
-                v += w * *reinterpret_cast<const f32x4*>(jo + ((w1 + i) * 16 + r) * OP + col);
-            }
-            if (a.nsplit == 1) {
-                const float inv = top == -INFINITY ? 0.f : 1.f / l;
-                if (col < a.D) store_out(a, row_at(a, b, hk, m) + col, v * inv);
-                if (col == 0 && a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(l)) * LN2;
-            } else {
-                const size_t at_row = (size_t)split * rows + (size_t)pair * a.M + m;
-                if (col < a.D) *reinterpret_cast<f32x4*>(a.ws + at_row * a.D + col) = v;
-                if (col == 0) {
-                    float* st = a.ws + (size_t)a.nsplit * rows * a.D + at_row * 2;
-                    st[0] = top;
-                    st[1] = l;
-                }
-            }
+            for (int i = 0; i < W; ++i) v += sm[w1 + i][row] * *reinterpret_cast<const f32x4*>(jo + ((w1 + i) * 16 + r) * OP + col);
+            if (a.nsplit == 1) store_out(a, out0 + (size_t)places[wave / W][row] * a.D + col, v);
+            else *reinterpret_cast<f32x4*>(a.ws + (row0 + row) * a.D + col) = v;
         }
     }
 }
@@ -546,9 +578,9 @@ __global__ void __launch_bounds__(256) k_xattn_delta(Args<T> a, float* delta) {
     }
 }
 
-// four values of dq: out, or to the key range's slab
-template <typename T> __device__ __forceinline__ void leave_dq(const Args<T>& a, int split, int pair, int b, int hk, int m, int col, f32x4 x) {
-    if (a.nsplit == 1) store4(a.dq + row_at(a, b, hk, m) + col, x);
+// four values of dq of row m, whose place is n: out, or to the key range's slab
+template <typename T> __device__ __forceinline__ void leave_dq(const Args<T>& a, int split, int pair, int b, int hk, int m, int n, int col, f32x4 x) {
+    if (a.nsplit == 1) store4(a.dq + pair_at(a, b, hk) + (size_t)n * a.D + col, x);
     else *reinterpret_cast<f32x4*>(a.ws + (((size_t)split * a.B * a.Hkv + pair) * a.M + m) * a.D + col) = x;
 }
 // four values of dk (which 0) or dv (1): out, or to the row range's slab [range][pair][dk | dv][key][D]
@@ -577,6 +609,7 @@ __global__ void __launch_bounds__(256, waves_bwd<T>(DF, MT)) k_xattn_bwd(Args<T>
     constexpr int PIECES = Y::NS * (Y::PARTS ? 2 : 1), SP = sizeof(T) == 4 ? 80 : 40, DS = PIECES * 16 * SP;     // dS^T: keys x 16 rows
     __shared__ __attribute__((aligned(16))) char lds[4 * TILE > JOIN ? 4 * TILE : JOIN];
     __shared__ __attribute__((aligned(16))) char lds_ds[4 * DS], rows_lds[HELD ? 16 : (4 / W) * 2 * ROWS];
+    __shared__ int places[4 / W][16 * MT];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4, w0 = wave % W;
     const int wi_ = work_item(a.blocks) * (4 / W) + wave / W;
     const bool idle = wi_ >= a.items;                        // an item past the last one: no keys, nothing stored
@@ -769,6 +802,8 @@ __global__ void __launch_bounds__(256, waves_bwd<T>(DF, MT)) k_xattn_bwd(Args<T>
     }
 
     float* jo = reinterpret_cast<float*>(lds);
+    const int it = threadIdx.x % (64 * W);                   // the thread in the item
+    if (it < 16 * MT) places[wave / W][it] = place_of(a, it);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         __syncthreads();
@@ -776,13 +811,14 @@ __global__ void __launch_bounds__(256, waves_bwd<T>(DF, MT)) k_xattn_bwd(Args<T>
         for (int d = 0; d < DT; ++d)
             *reinterpret_cast<f32x4*>(jo + (wave * 16 + li) * OP + d * 16 + g * 4) = dq[mt][d];
         __syncthreads();
-        for (int c = threadIdx.x % (64 * W); c < 16 * (DP / 4); c += 64 * W) {
+#pragma unroll 2
+        for (int c = it; c < 16 * (DP / 4); c += 64 * W) {
             const int r = c / (DP / 4), col = (c % (DP / 4)) * 4, m = mt * 16 + r;
             if (m >= M || col >= a.D) continue;
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < W; ++i) x += *reinterpret_cast<const f32x4*>(jo + ((wave - w0 + i) * 16 + r) * OP + col);
-            leave_dq(a, split, pair, b, hk, m, col, x);
+            leave_dq(a, split, pair, b, hk, m, places[wave / W][m], col, x);
         }
     }
 }
@@ -902,7 +938,7 @@ __global__ void __launch_bounds__(256, waves_bwd_q<T>(DF)) k_xattn_bwd_q(Args<T>
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < W; ++i) x += *reinterpret_cast<const f32x4*>(jo + ((wave - w0 + i) * 16 + r) * OP + col);
-            leave_dq(a, split, pair, b, hk, m, col, x * a.scale);
+            leave_dq(a, split, pair, b, hk, m, place_of(a, m), col, x * a.scale);
         }
     }
 }
@@ -1303,8 +1339,8 @@ template <int DF, int NW, int R = 64> struct RowTile {
         const unsigned per = D / 8, inv = (65536 + per - 1) / per;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const unsigned c = min((unsigned)(i * NW * 64 + threadIdx.x), per * R - 1), r = (c * inv) >> 16;
-            rc[i] = (int)(r | (c - r * per) << 8);
+            const unsigned c = min((unsigned)(i * NW * 64 + threadIdx.x), per * R - 1), r = __umul24(c, inv) >> 16;
+            rc[i] = (int)(r | (c - __umul24(r, per)) << 8);
         }
     }
     __device__ __forceinline__ unsigned row(int i) const { return rc[i] & 255; }
@@ -1377,8 +1413,8 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
         const Window kw = Tile::window(kb, a.k_st, key0, rows, a.D), vw = Tile::window(vb, a.v_st, key0, rows, a.D);
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) {
-            nxt.x[i] = kw.load((nxt.row(i) * (unsigned)a.k_st + nxt.col(i)) * 2u);
-            nxt.y[i] = vw.load((nxt.row(i) * (unsigned)a.v_st + nxt.col(i)) * 2u);
+            nxt.x[i] = kw.load(((__umul24(nxt.row(i), (unsigned)a.k_st >> 3) << 3) + nxt.col(i)) * 2u);
+            nxt.y[i] = vw.load(((__umul24(nxt.row(i), (unsigned)a.v_st >> 3) << 3) + nxt.col(i)) * 2u);
         }
     };
     load(first);
@@ -1391,14 +1427,14 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // scores stay unscaled, their maximum is found before the scale's product: that needs it positive (a negative one turns
-    // q's sign; of a zero, the least positive number makes the same weights)
-    const float scale2 = uniform(fmaxf(fabsf(a.scale) * LOG2E, 1e-37f));
-    if (a.scale < 0.f)
+    const float scale2 = positive_scale(a.scale);
+    if (a.scale < 0.f) {
+        rarely();
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int f = 0; f < DF; ++f) q[mt][f] = -q[mt][f];
+    }
     if (a.D < Tile::DP) { group_clear(lds, 4 * Tile::TILE); __syncthreads(); }
     unsigned long long on = live.bits(mask != nullptr, len, first * 64, lane), on_next = 0;
     nxt.put(lds, lds + Tile::TILE, on);
@@ -1543,8 +1579,8 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
         const Window kw = Tile::window(kb, a.k_st, key0, rows, a.D), vw = Tile::window(vb, a.v_st, key0, rows, a.D);
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) {
-            nxt.x[i] = kw.load((nxt.row(i) * (unsigned)a.k_st + nxt.col(i)) * 2u);
-            nxt.y[i] = vw.load((nxt.row(i) * (unsigned)a.v_st + nxt.col(i)) * 2u);
+            nxt.x[i] = kw.load(((__umul24(nxt.row(i), (unsigned)a.k_st >> 3) << 3) + nxt.col(i)) * 2u);
+            nxt.y[i] = vw.load(((__umul24(nxt.row(i), (unsigned)a.v_st >> 3) << 3) + nxt.col(i)) * 2u);
         }
     };
     load(first);
@@ -1610,7 +1646,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int col = d * 16 + g * 4;
-            if (col < a.D) leave_dq(a, split, pair, b, hk, m, col, dq[mt][d] * a.scale);
+            if (col < a.D) leave_dq(a, split, pair, b, hk, m, place_of(a, m), col, dq[mt][d] * a.scale);
         }
     }
 }
