@@ -99,7 +99,8 @@ SHAPES = [  # B, Tq, Tk, H, Hkv, D
     (1, 70, 300, 1, 1, 24), (2, 100, 513, 2, 2, 64), (1, 40, 260, 8, 2, 96), (1, 150, 321, 2, 1, 80), (1, 257, 700, 1, 1, 120),
     (2, 33, 449, 6, 2, 104), (1, 20, 385, 16, 2, 8),
     # more than 32 rows on at most 32 regions: the regions stay on the chip, whole and split rows
-    (3, 17, 1, 4, 2, 16), (2, 100, 5, 3, 3, 128), (1, 300, 16, 8, 2, 72), (1, 333, 17, 6, 3, 104), (2, 90, 32, 2, 1, 48), (5, 33, 23, 4, 4, 88)]
+    (3, 17, 1, 4, 2, 16), (2, 100, 5, 3, 3, 128), (1, 300, 16, 8, 2, 72), (1, 333, 17, 6, 3, 104), (2, 90, 32, 2, 1, 48), (5, 33, 23, 4, 4, 88),
+    (2, 20, 20, 3, 3, 64), (3, 24, 7, 1, 1, 128), (4, 16, 1, 2, 1, 104), (2, 9, 31, 4, 2, 32)]
 
 
 @pytest.mark.parametrize('B,Tq,Tk,H,Hkv,D', SHAPES)

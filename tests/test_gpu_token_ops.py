@@ -198,7 +198,7 @@ def test_refusals():
                  lambda: ops.cross_attention(torch.zeros(2, 3, 4, 136, **c), torch.zeros(2, 5, 2, 136, **c), torch.zeros(2, 5, 2, 136, **c)),
                  lambda: ops.cross_attention(q, k, k, mask=torch.ones(2, 4, dtype=torch.bool, **c)), lambda: ops.cross_attention(q, k, k, mask=torch.ones(2, 5, **c)),
                  lambda: ops.cross_attention(q, k, k, kv_len=torch.ones(2, dtype=torch.int32)),
-                 lambda: ops.cross_attention_bwd(o, q, k, k, o, None), lambda: ops.cross_attention_bwd(o[:, :2], q, k, k, o, saved)):
+                 lambda: ops.cross_attention(q, k, k, scale=float('nan')), lambda: ops.cross_attention_bwd(o, q, k, k, o, None), lambda: ops.cross_attention_bwd(o[:, :2], q, k, k, o, saved)):
         with pytest.raises(ValueError):
             call()
     for call in (lambda: ops.norm_gate(x.half()), lambda: ops.gated_scan(gates.double()), lambda: ops.cross_attention(q.half(), k.half(), k.half())):

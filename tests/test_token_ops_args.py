@@ -74,7 +74,7 @@ ATTN = dict(q=view(), k=view(), v=view(), kv_len=None, mask=None, mask_sb=0, sca
 @pytest.mark.parametrize('change', [dict(D=12), dict(D=136), dict(D=0), dict(H=3), dict(Hkv=0), dict(B=0), dict(Tq=0), dict(Tk=0), dict(dtype=4),
                                     dict(q=None), dict(k=view(data=None)), dict(v=view(data=P + 8)), dict(k=view(st=20)), dict(q=view(sb=-64)),
                                     dict(k=view(st=1 << 25)), dict(o=None), dict(o=P + 2), dict(rest=P + 2), dict(Tk=(1 << 24) + 1),
-                                    dict(Tq=1 << 27), dict(mask=P, mask_sb=-4), dict(B=1, Tk=100000)])
+                                    dict(Tq=1 << 27), dict(mask=P, mask_sb=-4), dict(B=1, Tk=100000), dict(scale=float('nan')), dict(scale=float('-inf'))])
 def test_attention_forward_refuses(change):
     refused('vqa_cross_attn_fwd', *{**ATTN, **change}.values())
 
@@ -83,7 +83,7 @@ def test_attention_backward_refuses():
     ok = dict(do=P, q=view(), k=view(), v=view(), o=P, rest=None, lse=P, kv_len=None, mask=None, mask_sb=0, scale=0.25, dq=P, dk=P, dv=P, ws=P, B=2,
               Tq=3, Tk=16, H=4, Hkv=2, D=16, dtype=1)
     for change in (dict(do=None), dict(o=None), dict(lse=None), dict(dq=None), dict(dk=P + 4), dict(dv=None), dict(D=10), dict(v=view(st=4)),
-                   dict(Tq=40, Tk=64, ws=None), dict(ws=P + 4), dict(rest=P + 4)):
+                   dict(Tq=40, Tk=64, ws=None), dict(ws=P + 4), dict(rest=P + 4), dict(scale=float('inf'))):
         refused('vqa_cross_attn_bwd', *{**ok, **change}.values())
 
 
@@ -94,7 +94,7 @@ def test_workspace_sizes():
     assert lib.vqa_norm_gate_workspace_floats(100, 64, 0) >= 3 * 64 and lib.vqa_norm_gate_workspace_floats(100, 64, 7) == 0
     assert lib.vqa_cross_attn_fwd_workspace_floats(256, 14, 196, 15, 15, 80, 1) == 0
     assert lib.vqa_cross_attn_fwd_workspace_floats(1, 1, 4096, 8, 2, 64, 1) > 0
-    assert lib.vqa_cross_attn_bwd_workspace_floats(2, 40, 64, 4, 2, 64, 0) == 2 * 40 * 4
+    assert lib.vqa_cross_attn_bwd_workspace_floats(2, 40, 64, 4, 2, 64, 0) >= 2 * 40 * 4
     assert lib.vqa_cross_attn_fwd_workspace_floats(1, 1, 4096, 8, 3, 64, 1) == 0        # sizes that are refused
 
 

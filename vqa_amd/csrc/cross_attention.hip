@@ -2073,7 +2073,8 @@ bool sizes_ok(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
                 "D a multiple of 8 up to 128, B * Tq * H <= 2^27, Tk <= 2^24");                                                 \
     VQA_REQUIRE(q && k && v && view_ok(*q) && view_ok(*k) && view_ok(*v),                                                      \
                 fn ": q, k, v must be 16-byte aligned with strides that are multiples of 8");                                  \
-    VQA_REQUIRE(!mask || B == 1 || mask_sb >= 0, fn ": the mask's stride must not be negative");
+    VQA_REQUIRE(!mask || B == 1 || mask_sb >= 0, fn ": the mask's stride must not be negative");                               \
+    VQA_REQUIRE(isfinite(scale), fn ": scale must be finite");
 
 }  // namespace
 

@@ -13,6 +13,7 @@ the kernels cannot read in 16-byte pieces (odd strides or addresses) is copied f
 from __future__ import annotations
 
 import functools
+import math
 from ctypes import byref
 
 import torch
@@ -335,7 +336,9 @@ def _attn_operands(q, k, v, kv_len, mask, scale):
         if Tk > 1 and mask.stride(1) != 1:
             mask = mask.contiguous()
         mask_sb = mask.stride(0)
-    return dt, _lengths(name, 'kv_len', kv_len, q, B), mask, mask_sb, D ** -0.5 if scale is None else float(scale), B, Tq, Tk, H, Hkv, D
+    scale = D ** -0.5 if scale is None else float(scale)
+    _need(math.isfinite(scale), '{}: scale must be finite, got {}', name, scale)
+    return dt, _lengths(name, 'kv_len', kv_len, q, B), mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D
 
 
 def cross_attention_fwd(q, k, v, kv_len=None, mask=None, scale=None, save=True):
@@ -343,7 +346,7 @@ def cross_attention_fwd(q, k, v, kv_len=None, mask=None, scale=None, save=True):
     reads key head h // (H // Hkv).
 
     ``kv_len`` (B,): regions of each sample; ``mask`` (B, Tk): regions that count (True); what does not count
-    may hold anything.  ``scale`` defaults to D ** -0.5.  Returns o (B, Tq, H, D), a row with nothing to attend 0, and what
+    may hold anything.  ``scale`` (finite) defaults to D ** -0.5.  Returns o (B, Tq, H, D), a row with nothing to attend 0, and what
     ``cross_attention_bwd`` needs (None unless ``save``): the log-sum-exp of the scores (B, H, Tq) float32, -inf for such a
     row, and for bfloat16 what rounding took from o."""
     dt, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D = _attn_operands(q, k, v, kv_len, mask, scale)
