@@ -1327,8 +1327,11 @@ __global__ void __launch_bounds__(256) k_xattn_dkv_join(Args<T> a) {
 // Beyond 64 rows and 256 keys the matrix cores are the bound (14 M Tk / (M + Tk) flops per byte and 16-bit element, against
 // 230 that the card does per byte it reads), and what feeds them is LDS: a wave that reads a 16 x 16 key fragment once for
 // two row tiles keeps LDS as busy as the matrix core.  Keys (rows, in the keys' backward) lie in LDS, two tiles of 64, for
-// eight waves of 32 rows each; the next tile is in flight in registers.  P and dS are rounded to bf16 for their products
-// (2^-9 of every term at random, over more than 256 terms).
+// eight waves of 32 rows each; the next tile is in flight in registers.  P and dS are rounded to bf16 for their products:
+// as much noise, over more than 256 terms, as the rounding of the result, sqrt(2) of its error together.  dq alone has more
+// where rows are short: its terms dS k cancel down to dS (k - k'), k' the keys' weighted mean, whose share of k is 1 / D with
+// independent keys, while the noise is that of dS k (1.5 of the rounding's error at D <= 32, 1.43 from 64 on).  Up to 64 its
+// dS therefore comes in two parts (8 x 509 on 2000 x 8 heads of 64: 56 us instead of 46).
 
 // R rows (64 or 32) of two operands on their way to LDS, NW waves together
 template <int DF, int NW, int R = 64> struct RowTile {
@@ -1546,6 +1549,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
     typedef Ty<bf16_t> Y;
     typedef RowTile<DF, NW> Tile;
     constexpr int DT = DF * 2, PITCH = Tile::PITCH, MT = 2;
+    constexpr bool TWO = DF <= 2;                            // dS in two parts
     __shared__ __attribute__((aligned(16))) char lds[4 * Tile::TILE];
     const int wi = work_item(a.blocks);
     if (wi >= a.blocks) return;
@@ -1602,7 +1606,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
         if (on)                                              // (a tile that is masked throughout adds nothing)
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            Y::half h[MT][2];
+            Y::half h[MT][2], lo[MT][2];
 #pragma unroll
             for (int ns = 0; ns < 2; ++ns) {
                 const int sub = kk * 2 + ns;
@@ -1624,13 +1628,17 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_q_tile(Args<bf16_t> a) {
                     for (int r = 0; r < 4; ++r)              // (a key that does not count is a row of zeros: its ds need only be finite)
                         dp[mt][r] = __builtin_amdgcn_exp2f(fminf(s[mt][r] * scale2 - lse[mt], 1.f)) * (dp[mt][r] - delta[mt]);
                     h[mt][ns] = Y::pack(dp[mt]);
+                    if (TWO) lo[mt][ns] = Y::rest(dp[mt], h[mt][ns]);
                 }
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const bf16x8_t kt = frag_t<bf16_t>(lk + kk * 32 * PITCH, PITCH, d * 16, li, g);
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) dq[mt][d] = Y::mma(kt, Y::join(h[mt]), dq[mt][d]);
+                for (int mt = 0; mt < MT; ++mt) {
+                    dq[mt][d] = Y::mma(kt, Y::join(h[mt]), dq[mt][d]);
+                    if (TWO) dq[mt][d] = Y::mma(kt, Y::join(lo[mt]), dq[mt][d]);
+                }
             }
         }
         cur ^= 1;
