@@ -74,7 +74,8 @@ ATTN = dict(q=view(), k=view(), v=view(), kv_len=None, mask=None, mask_sb=0, sca
 @pytest.mark.parametrize('change', [dict(D=12), dict(D=136), dict(D=0), dict(H=3), dict(Hkv=0), dict(B=0), dict(Tq=0), dict(Tk=0), dict(dtype=4),
                                     dict(q=None), dict(k=view(data=None)), dict(v=view(data=P + 8)), dict(k=view(st=20)), dict(q=view(sb=-64)),
                                     dict(k=view(st=1 << 25)), dict(o=None), dict(o=P + 2), dict(rest=P + 2), dict(Tk=(1 << 24) + 1),
-                                    dict(Tq=1 << 27), dict(mask=P, mask_sb=-4), dict(B=1, Tk=100000), dict(scale=float('nan')), dict(scale=float('-inf'))])
+                                    dict(Tq=1 << 27), dict(mask=P, mask_sb=-4), dict(B=1, Tk=100000), dict(scale=float('nan')), dict(scale=float('-inf')),
+                                    dict(B=1 << 23, Tq=1), dict(B=1 << 17, Tq=1, Tk=3000)])
 def test_attention_forward_refuses(change):
     refused('vqa_cross_attn_fwd', *{**ATTN, **change}.values())
 

@@ -2074,11 +2074,13 @@ int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
 bool sizes_ok(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
     return (dtype == VQA_F32 || dtype == VQA_BF16) && B > 0 && Tq > 0 && Tk > 0 && Hkv > 0 && H > 0 && H % Hkv == 0 && D > 0 &&
            D % 8 == 0 && D <= VQA_CROSS_ATTN_MAX_D && (long)B * Tq * H <= (1L << 27) && Tk <= (1 << 24) &&
-           (long)B * Hkv * ((Tk + 63) / 64) <= (1L << 28) && (long)Hkv * D < (1L << 25);
+           (long)Hkv * D < (1L << 25) &&
+           // (a launch has fewer than 2^32 threads; the largest grids are these blocks, of 256)
+           (long)B * Hkv * (((long)Tq * (H / Hkv) + 15) / 16) <= (1L << 23) && (long)B * Hkv * ((Tk + 63) / 64) <= (1L << 23);
 }
 #define XA_COMMON(fn)                                                                                                          \
     VQA_REQUIRE(sizes_ok(B, Tq, Tk, H, Hkv, D, dtype), fn ": dtype VQA_F32 or VQA_BF16, positive sizes, H a multiple of Hkv, " \
-                "D a multiple of 8 up to 128, B * Tq * H <= 2^27, Tk <= 2^24");                                                 \
+                "D a multiple of 8 up to 128, B * Tq * H <= 2^27, Tk <= 2^24, at most 2^23 blocks of 16 rows or 64 keys");      \
     VQA_REQUIRE(q && k && v && view_ok(*q) && view_ok(*k) && view_ok(*v),                                                      \
                 fn ": q, k, v must be 16-byte aligned with strides that are multiples of 8");                                  \
     VQA_REQUIRE(!mask || B == 1 || mask_sb >= 0, fn ": the mask's stride must not be negative");                               \
