@@ -1854,10 +1854,15 @@ int fwd_splits(int B, int Tq, int Tk, int H, int Hkv, int D, int dtype) {
 }
 int bwd_splits(int B, int Tq, int Tk, int H, int Hkv, int dtype) { return key_splits((long)B * Hkv, Tk, dtype, false); }
 
-// Waves per work item: two, so that an item's end (the join) and the next one's beginning overlap with other items; four
-// where the items are fewer than two to a CU and only their own length counts (one image of 196 regions: 5.6 against 7.2 us,
-// 256 images x 15 heads: 66 against 61 us)
-int waves_of(const int items) { return items < 512 ? 4 : 2; }
+// Waves per work item: two, so that an item's end (the join) and the next one's beginning overlap with other items (64 x 8
+// rows on 700 x 8 heads: 17 against 21 us); four where the items are fewer than two to a CU and only their own length counts
+// (one image of 196 regions: 5.6 against 7.2), and where two would fill a last round of CUs by less than half (150 x 1 row
+// on 1000 x 8 heads of 128, fp32: 229 against 243 forward, 440 against 493 backward; 40 x 60 on 700: 50 against 64), if an item is
+// `least` tiles long.
+int waves_of(const int items, const int tiles, const int least) {
+    return items < 512 || (tiles >= least && (items - 1) % 512 < 256 && items <= 2816) ? 4 : 2;
+}
+constexpr int LEAST_FWD = 5, LEAST_BWD = 9, LEAST_Q = 16;     // forward, one-pass backward, dq of many rows
 
 // The two-kernel backward: blocks, key ranges of the dq kernel, row ranges of the dk / dv kernel.  Ranges only where the
 // blocks alone leave CUs idle; row ranges of at least 4 tiles, at most 16 (slabs of dk and dv are as large as they are).
@@ -1886,7 +1891,7 @@ TwoPlan two_plan(int B, int Hkv, long M, int Tk, int D, int dtype) {
 
 template <typename T, int DF, int MT> void launch_fwd(const Args<T>& a, hipStream_t s) {
     const int grid = 8 * ((a.blocks + 7) / 8);
-    if (waves_of(a.items) == 2) k_xattn_fwd<T, DF, MT, 2><<<grid, 256, 0, s>>>(a);
+    if (waves_of(a.items, a.tiles_split, LEAST_FWD) == 2) k_xattn_fwd<T, DF, MT, 2><<<grid, 256, 0, s>>>(a);
     else k_xattn_fwd<T, DF, MT, 4><<<grid, 256, 0, s>>>(a);
 }
 template <typename T, int DF> void launch_fwd_mt(const Args<T>& a, int mt, hipStream_t s) {
@@ -1896,7 +1901,7 @@ template <typename T, int DF> void launch_fwd_mt(const Args<T>& a, int mt, hipSt
 }
 template <typename T, int DF> void launch_bwd(const Args<T>& a, hipStream_t s) {
     const int grid = 8 * ((a.blocks + 7) / 8);
-    if (waves_of(a.items) == 2) {
+    if (waves_of(a.items, a.tiles_split, LEAST_BWD) == 2) {
         if (a.M > 16) k_xattn_bwd<T, DF, 2, 2><<<grid, 256, 0, s>>>(a);
         else k_xattn_bwd<T, DF, 1, 2><<<grid, 256, 0, s>>>(a);
     } else {
@@ -1906,7 +1911,7 @@ template <typename T, int DF> void launch_bwd(const Args<T>& a, hipStream_t s) {
 }
 template <typename T, int DF> void launch_bwd_q(const Args<T>& a, hipStream_t s) {
     const int grid = 8 * ((a.blocks + 7) / 8);
-    if (waves_of(a.items) == 2) k_xattn_bwd_q<T, DF, 2, 2><<<grid, 256, 0, s>>>(a);
+    if (waves_of(a.items, a.tiles_split, LEAST_Q) == 2) k_xattn_bwd_q<T, DF, 2, 2><<<grid, 256, 0, s>>>(a);
     else k_xattn_bwd_q<T, DF, 2, 4><<<grid, 256, 0, s>>>(a);
 }
 
@@ -1990,7 +1995,7 @@ int fwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
         const int tiles = (a.Tk + Ty<T>::KC - 1) / Ty<T>::KC;
         a.tiles_split = (tiles + nsplit - 1) / nsplit;
         a.items = a.B * a.Hkv * a.row_blocks * nsplit;
-        a.blocks = waves_of(a.items) == 2 ? (a.items + 1) / 2 : a.items;
+        a.blocks = waves_of(a.items, a.tiles_split, LEAST_FWD) == 2 ? (a.items + 1) / 2 : a.items;
         BY_WIDTH(T, a.D, (launch_fwd_mt<T, DF>(a, mt, stream)));
     }
     int rc = vqa_check_launch("vqa_cross_attn_fwd");
@@ -2007,7 +2012,7 @@ int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
         const int tiles = (a.Tk + Ty<T>::KC - 1) / Ty<T>::KC;
         a.tiles_split = (tiles + nsplit - 1) / nsplit;
         a.items = a.B * a.Hkv * nsplit;
-        a.blocks = waves_of(a.items) == 2 ? (a.items + 1) / 2 : a.items;
+        a.blocks = waves_of(a.items, a.tiles_split, LEAST_BWD) == 2 ? (a.items + 1) / 2 : a.items;
         BY_WIDTH(T, a.D, (launch_bwd<T, DF>(a, stream)));
         int rc = vqa_check_launch("vqa_cross_attn_bwd");
         if (rc || nsplit == 1) return rc;
@@ -2046,7 +2051,7 @@ int bwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
         }
     }
     if (!tile) {
-        a.blocks = waves_of(a.items) == 2 ? (a.items + 1) / 2 : a.items;
+        a.blocks = waves_of(a.items, a.tiles_split, LEAST_Q) == 2 ? (a.items + 1) / 2 : a.items;
         BY_WIDTH(T, a.D, (launch_bwd_q<T, DF>(a, stream)));
     }
     int rc = vqa_check_launch("vqa_cross_attn_bwd (dq)");
