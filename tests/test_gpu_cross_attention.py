@@ -177,6 +177,28 @@ def test_scores_far_below_zero_and_signs_of_the_scale(shape, scale):
     _check(q, k, v, do, kv_len=torch.full((B,), Tk - 5, device='cuda', dtype=torch.int32), mask=mask, scale=scale)
 
 
+@pytest.mark.parametrize('shape', [(2, 7, 90, 2, 2, 64), (2, 40, 70, 4, 2, 64), (2, 90, 400, 2, 2, 64), (2, 40, 20, 3, 1, 64), (2, 20, 60, 1, 1, 24)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_an_infinite_output_gradient_stays_with_what_counts(shape, dtype):
+    """dO infinite in one row of the first sample: regions that do not count keep zero gradients there, a sample with nothing
+    to attend keeps its own at zero, the other sample is untouched."""
+    from vqa_amd import ops
+    q, k, v, do = _inputs(*shape, dtype, 12, fused=False)
+    mask = torch.rand(2, shape[2], device='cuda', generator=torch.Generator(device='cuda').manual_seed(4)) < 0.5
+    o, saved = ops.cross_attention_fwd(q, k, v, mask=mask)
+    clean = ops.cross_attention_bwd(do, q, k, v, o, saved, mask=mask)
+    do[0, 1] = float('inf')
+    got = ops.cross_attention_bwd(do, q, k, v, o, saved, mask=mask)
+    for a, b in zip(got, clean):
+        assert torch.equal(a[1], b[1])
+    for x in got[1:]:
+        assert float(x[~mask].abs().sum()) == 0
+    assert not bool(torch.isfinite(got[2][0][mask[0]]).any())
+    none = torch.zeros_like(mask)
+    o, saved = ops.cross_attention_fwd(q, k, v, mask=none)
+    assert all(float(x.abs().sum()) == 0 for x in (o, *ops.cross_attention_bwd(do, q, k, v, o, saved, mask=none)))
+
+
 def test_infinite_and_nan_operands_spread_as_in_the_formula():
     from vqa_amd import ops
     q, k, v, do = _inputs(2, 3, 40, 2, 2, 16, torch.float32, 3, fused=False)

@@ -122,7 +122,7 @@ __device__ __forceinline__ void wave_lds_order() {
 // Waves per SIMD that a kernel of this file is compiled for: two, which leaves it 256 registers and products that add up in
 // ordinary ones; with one it gets 512, but the products' sums move to the accumulation registers and back for every use
 // (96-wide rows, 64 x 60 on 200 x 8 heads, bf16: dq 23.7 -> 18.6 us, dk / dv 43.8 -> 33.4; fp32 dq 56.7 -> 46.3).  One where
-// 256 do not suffice and the rest would go to memory (128-wide: dq 30.6, with two 40.2; 96-wide forward of 64 rows 23 and 46).
+// 256 do not suffice and much of the rest would go to memory (dk / dv's few words cost less; 128-wide: dq 30.6, with two 40.2; 96-wide forward of 64 rows 23 and 46).
 template <typename T> constexpr int waves_fwd(int df, int mt) { return sizeof(T) == 2 ? (df * mt > 8 ? 1 : 2) : (df * mt > 12 ? 1 : 2); }
 template <typename T> constexpr int waves_bwd(int df, int mt) { return df * (mt + 1) > (sizeof(T) == 2 ? 6 : 8) ? 1 : 2; }
 template <typename T> constexpr int waves_bwd_q(int df) { return df > (sizeof(T) == 2 ? 3 : 6) ? 1 : 2; }
@@ -793,9 +793,18 @@ __global__ void __launch_bounds__(256, waves_bwd<T>(DF, MT)) k_xattn_bwd(Args<T>
             wave_lds_order();
             const int n = min(Y::KC, a.Tk - key0);
             const Window w(to + (((size_t)b * a.Tk + key0) * a.Hkv + hk) * a.D, ((n - 1) * out_st + a.D) * (unsigned)sizeof(T));
+            u32x4 out[DT];
 #pragma unroll
-            for (int i = 0; i < DT; ++i)
-                w.store(sp.at(i, out_st), *reinterpret_cast<const u32x4*>(my + sp.row(i) * PITCH + sp.col(i) * (int)sizeof(T)));
+            for (int i = 0; i < DT; ++i) out[i] = *reinterpret_cast<const u32x4*>(my + sp.row(i) * PITCH + sp.col(i) * (int)sizeof(T));
+            const unsigned on = bits.b[0] | bits.b[Y::NS - 1] << (16 * (Y::NS - 1));
+            if (on != (Y::NS == 2 ? 0xffffffffu : 0xffffu)) {            // keys that do not count: 0, whatever dO holds
+                rarely();
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+                    if (!((on >> sp.row(i)) & 1)) out[i] = u32x4{};
+            }
+#pragma unroll
+            for (int i = 0; i < DT; ++i) w.store(sp.at(i, out_st), out[i]);
         };
         leave(a.dv, do_t, ldo, p, p_lo);
         leave(a.dk, q_t, lq, ds, ds_lo);
@@ -1049,12 +1058,14 @@ __global__ void __launch_bounds__(256, 2) k_xattn_bwd_kv(Args<T> a) {
     for (int ns = 0; ns < Y::NS; ++ns) {
         const int key = key0 + ns * 16 + li;
         if (key >= a.Tk) continue;
+        const bool on = (bits.b[ns] >> li) & 1;              // (a key that does not count: 0, whatever dO holds)
+        const f32x4 z = {};
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int c = d * 16 + g * 4;
             if (c < a.D) {
-                leave_dkv(a, split, pair, 0, key, c, dk[ns][d] * a.scale);
-                leave_dkv(a, split, pair, 1, key, c, dv[ns][d]);
+                leave_dkv(a, split, pair, 0, key, c, on ? dk[ns][d] * a.scale : z);
+                leave_dkv(a, split, pair, 1, key, c, on ? dv[ns][d] : z);
             }
         }
     }
@@ -1305,7 +1316,7 @@ __global__ void __launch_bounds__(256, waves_bwd_few<T>(DF, NK)) k_xattn_bwd_few
                 f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x += *reinterpret_cast<const f32x4*>(jo + (i * 16 + r) * OP + col);
-                leave_dkv(a, split, pair, which, key, col, x);
+                leave_dkv(a, split, pair, which, key, col, (on >> key) & 1 ? x : f32x4{0.f, 0.f, 0.f, 0.f});
             }
         }
 }
