@@ -47,6 +47,17 @@ def _entry(name):
     return getattr(_lib.load(), name)
 
 
+@functools.lru_cache(1024)
+def _floats(name, *sizes):
+    """What a workspace-size function says for these sizes (a foreign call costs as much as an allocation)."""
+    return _entry(name)(*sizes)
+
+
+def _new(t):
+    """An uninitialised, contiguous tensor like `t` (None for None)."""
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -111,12 +122,12 @@ def gated_scan_fwd(gates, lengths=None, c0=None, save=True):
     ``save``).  With T = 1 and ``c0`` the state of the last call this is one step of a running sequence."""
     dt, gates, sb, st, lengths, c0, B, T, H = _scan_operands(gates, lengths, c0, 'gated_scan')
     dev = gates.device
-    h = torch.empty((B, T, H), dtype=gates.dtype, device=dev)
-    c = torch.empty((B, H), dtype=torch.float32, device=dev)
-    saved = torch.empty(((T + _SAVE - 1) // _SAVE, B, H), dtype=torch.float32, device=dev) if save else None
+    h = gates.new_empty((B, T, H))
+    c = gates.new_empty((B, H), dtype=torch.float32)
+    saved = gates.new_empty(((T + _SAVE - 1) // _SAVE, B, H), dtype=torch.float32) if save else None
     if B == 0 or T == 0 or H == 0:
         return h, c.zero_() if c0 is None else c.copy_(c0), saved
-    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H, dt), dev)
+    ws = _workspace(_floats('vqa_gated_scan_workspace_floats', B, T, H, dt), gates)
     _call(dev, 'vqa_gated_scan_fwd', gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0), h.data_ptr(), c.data_ptr(),
           _ptr(saved), _ptr(ws), B, T, H, dt)
     return h, c, saved
@@ -127,8 +138,8 @@ def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
     the gradient at the last state (either may be None: zero)."""
     dt, gates, sb, st, lengths, c0, B, T, H = _scan_operands(gates, lengths, c0, 'gated_scan')
     dev = gates.device
-    dgates = torch.empty((B, T, 4 * H), dtype=gates.dtype, device=dev)
-    dc0 = torch.empty((B, H), dtype=torch.float32, device=dev)
+    dgates = _new(gates)
+    dc0 = gates.new_empty((B, H), dtype=torch.float32)
     if dh is not None:
         _like('gated_scan', 'dh', dh, gates, (B, T, H))
         dh = _packed(dh)
@@ -139,7 +150,7 @@ def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
         return dgates.zero_(), dc0.zero_() if dc is None else dc0.copy_(dc)
     _need(saved is not None and tuple(saved.shape) == ((T + _SAVE - 1) // _SAVE, B, H),
           'gated_scan: the backward needs what gated_scan_fwd(..., save=True) returned for these gates')
-    ws = _workspace(_entry('vqa_gated_scan_workspace_floats')(B, T, H, dt), dev)
+    ws = _workspace(_floats('vqa_gated_scan_workspace_floats', B, T, H, dt), gates)
     _call(dev, 'vqa_gated_scan_bwd', _ptr(dh), _ptr(dc), gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0),
           saved.data_ptr(), dgates.data_ptr(), dc0.data_ptr(), _ptr(ws), B, T, H, dt)
     return dgates, dc0
@@ -148,10 +159,10 @@ def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
 _SAVE = 8                    # VQA_GATED_SCAN_SAVE of include/vqa_hip.h
 
 
-def _workspace(floats, device):
+def _workspace(floats, like):
     """Scratch of one call, from torch's allocator: it belongs to the stream of the call (and, under capture, to the
     graph), so calls on two streams and two captured graphs never share it."""
-    return torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+    return like.new_empty(floats, dtype=torch.float32) if floats else None
 
 
 class _GatedScan(torch.autograd.Function):
@@ -241,9 +252,9 @@ def norm_gate_fwd(x, f=None, gate=None, residual_scale=None, w_post=None, w_pre=
     want_y = want_y and f is not None
     _need(want_y or want_h, '{}: one of y, h must be wanted', name)
     _need(want_h or w_pre is None, '{}: w_pre belongs to h', name)
-    y = torch.empty_like(x, memory_format=torch.contiguous_format) if want_y else None
-    h = torch.empty_like(x, memory_format=torch.contiguous_format) if want_h else None
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if save else None
+    y = _new(x) if want_y else None
+    h = _new(x) if want_h else None
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if save else None
     if rows == 0:
         return y, h, stats
     (x, ldx), (f, ldf), (gate, ldg) = _rows(x), _rows(f), _rows(gate)
@@ -265,11 +276,8 @@ def norm_gate_bwd(dy, dh, x, stats, f=None, gate=None, residual_scale=None, w_po
             _like(name, what, g, x, x.shape)
     _like(name, 'stats', stats, x, (rows, 2), torch.float32)
 
-    def new(t, dtype=None):
-        return None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=x.device)
-
-    dx, df, dgate = new(x), new(f), new(gate)
-    drho, dw_post, dw_pre = new(residual_scale), new(w_post), new(w_pre)
+    dx, df, dgate = _new(x), _new(f), _new(gate)
+    drho, dw_post, dw_pre = _new(residual_scale), _new(w_post), _new(w_pre)
     if rows == 0:
         for g in (drho, dw_post, dw_pre, dgate):
             if g is not None:
@@ -277,7 +285,7 @@ def norm_gate_bwd(dy, dh, x, stats, f=None, gate=None, residual_scale=None, w_po
         return dx, df, dgate, drho, dw_post, dw_pre
     (x, ldx), (f, ldf), (gate, ldg), (dy, lddy), (dh, lddh) = _rows(x), _rows(f), _rows(gate), _rows(dy), _rows(dh)
     rho, w_post, w_pre, stats = _packed(residual_scale), _packed(w_post), _packed(w_pre), _packed(stats)
-    ws = _workspace(_entry('vqa_norm_gate_workspace_floats')(rows, D, per), x.device)
+    ws = _workspace(_floats('vqa_norm_gate_workspace_floats', rows, D, per), x)
     _call(x.device, 'vqa_norm_gate_bwd', _ptr(dy), lddy, _ptr(dh), lddh, x.data_ptr(), ldx, _ptr(f), ldf, _ptr(gate), ldg, per,
           _ptr(rho), _ptr(w_post), _ptr(w_pre), stats.data_ptr(), dx.data_ptr(), D, _ptr(df), D, _ptr(dgate), D,
           _ptr(drho), _ptr(dw_post), _ptr(dw_pre), ws.data_ptr(), rows, D, dt)
@@ -351,13 +359,13 @@ def cross_attention_fwd(q, k, v, kv_len=None, mask=None, scale=None, save=True):
     row, and for bfloat16 what rounding took from o."""
     dt, kv_len, mask, mask_sb, scale, B, Tq, Tk, H, Hkv, D = _attn_operands(q, k, v, kv_len, mask, scale)
     dev = q.device
-    o = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, H, Tq), dtype=torch.float32, device=dev) if save else None
-    rest = torch.empty_like(o) if save and dt == _lib.BF16 else None
+    o = _new(q)
+    lse = q.new_empty((B, H, Tq), dtype=torch.float32) if save else None
+    rest = _new(q) if save and dt == _lib.BF16 else None
     if B == 0 or Tq == 0 or Tk == 0:
         return o.zero_(), (lse.fill_(float('-inf')), rest if rest is None else rest.zero_()) if save else None
     (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
-    ws = _workspace(_entry('vqa_cross_attn_fwd_workspace_floats')(B, Tq, Tk, H, Hkv, D, dt), dev)
+    ws = _workspace(_floats('vqa_cross_attn_fwd_workspace_floats', B, Tq, Tk, H, Hkv, D, dt), q)
     _call(dev, 'vqa_cross_attn_fwd', byref(vq), byref(vk), byref(vv), _ptr(kv_len), _ptr(mask), mask_sb, scale, o.data_ptr(),
           _ptr(rest), _ptr(lse), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
     return o, (lse, rest) if save else None
@@ -374,13 +382,12 @@ def cross_attention_bwd(do, q, k, v, o, saved, kv_len=None, mask=None, scale=Non
     _like('cross_attention', 'the saved log-sum-exp', lse, q, (B, H, Tq), torch.float32)
     if rest is not None:
         _like('cross_attention', "the saved rest of o", rest, q, q.shape)
-    dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=dev)
-    dk, dv = (torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=dev) for _ in range(2))
+    dq, dk, dv = _new(q), _new(k), _new(v)
     if B == 0 or Tq == 0 or Tk == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     (q, vq), (k, vk), (v, vv) = _view(q), _view(k), _view(v)
     do, o, lse, rest = _packed(do), _packed(o), _packed(lse), _packed(rest)
-    ws = _workspace(_entry('vqa_cross_attn_bwd_workspace_floats')(B, Tq, Tk, H, Hkv, D, dt), dev)
+    ws = _workspace(_floats('vqa_cross_attn_bwd_workspace_floats', B, Tq, Tk, H, Hkv, D, dt), q)
     _call(dev, 'vqa_cross_attn_bwd', do.data_ptr(), byref(vq), byref(vk), byref(vv), o.data_ptr(), _ptr(rest), lse.data_ptr(),
           _ptr(kv_len), _ptr(mask), mask_sb, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), B, Tq, Tk, H, Hkv, D, dt)
     return dq, dk, dv
