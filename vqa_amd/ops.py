@@ -213,27 +213,31 @@ def _rows(t):
 
 
 def _norm_operands(name, x, f, gate, residual_scale, w_post, w_pre):
-    dt = _storage(name, x)
-    D = x.shape[-1] if x.dim() else 0
+    dt, shape = _storage(name, x), x.shape
+    D = shape[-1] if shape else 0
     _need(D % 8 == 0 and 8 <= D <= 8192, '{}: the width must be a multiple of 8 in [8, 8192]', name)
     rows = x.numel() // D
     if f is not None:
-        _like(name, 'f', f, x, x.shape)
+        _like(name, 'f', f, x, shape)
     elif gate is not None or residual_scale is not None or w_post is not None:
         raise ValueError(f'{name}: gate, residual_scale and w_post belong to the block output f')
     per = 0
     if gate is not None:
-        per = 1
-        if gate.shape != x.shape:
+        per, gs = 1, gate.shape
+        if gs != shape:
             # the gate's leading dimensions are x's up to some point, then ones: row r belongs to gate row r // per
-            lead, full = list(gate.shape[:-1]), list(x.shape[:-1])
-            cut = max([i + 1 for i, s in enumerate(lead) if s != 1], default=0)
-            _need(gate.dim() and gate.shape[-1] == D and len(lead) <= len(full) and lead[:cut] == full[:cut],
-                  '{}: gate {} must share the leading dimensions of x {} up to some point and have size 1 behind it',
-                  name, tuple(gate.shape), tuple(x.shape))
-            n = gate.numel() // D
-            per = rows // n if n else 1
-        _like(name, 'gate', gate, x, gate.shape)
+            if len(gs) == 3 == len(shape) and gs[0] == shape[0] and gs[1] == 1 and gs[2] == D:
+                per = shape[1]
+            else:
+                lead, full = list(gs[:-1]), list(shape[:-1])
+                cut = max([i + 1 for i, s in enumerate(lead) if s != 1], default=0)
+                _need(len(gs) and gs[-1] == D and len(lead) <= len(full) and lead[:cut] == full[:cut],
+                      '{}: gate {} must share the leading dimensions of x {} up to some point and have size 1 behind it',
+                      name, tuple(gs), tuple(shape))
+                n = gate.numel() // D
+                per = rows // n if n else 1
+            per = max(per, 1)
+        _like(name, 'gate', gate, x, gs)
     for what, w in (('residual_scale', residual_scale), ('w_post', w_post), ('w_pre', w_pre)):
         if w is not None:
             _like(name, what, w, x, (D,), torch.float32)
