@@ -16,8 +16,8 @@
 //   64 x 1 row x 8 key heads of 128 (4 query heads each) on 4096 regions, ragged: 155 us, at the copy rate (5.1 TB/s)
 //   256 x 14 on 196 x 15 heads of 80, ragged: forward 55 - 65 us, backward 97 - 103 us
 // with many rows and regions the matrix cores:
-//   8 x 509 on 4096 x 8 key heads of 128 (2 each): forward 165 us (830 TFLOP/s), dq 203 us (three products, 1010 TFLOP/s),
-//   dk and dv 325 us (four products, 840 TFLOP/s); a large library product reaches 1180 there
+//   8 x 509 on 4096 x 8 key heads of 128 (2 each): forward 163 us (840 TFLOP/s), dq 201 us (three products, 1020 TFLOP/s),
+//   dk and dv 321 us (four products, 850 TFLOP/s); a large library product reaches 1180 there
 // and fp32 32 x 20 on 576 x 8 heads of 64: 21 and 42 us.  The variants, by rules of two_plan(), few(), one_pass(), tiled():
 // k_xattn_fwd / k_xattn_bwd stream the keys past up to 64 (32) rows in registers; k_xattn_bwd_q / _bwd_kv for more rows;
 // k_xattn_*_tile for more than 64 rows on more than 256 keys; k_xattn_*_few for at most 32 keys.
