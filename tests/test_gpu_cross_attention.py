@@ -199,6 +199,24 @@ def test_an_infinite_output_gradient_stays_with_what_counts(shape, dtype):
     assert all(float(x.abs().sum()) == 0 for x in (o, *ops.cross_attention_bwd(do, q, k, v, o, saved, mask=none)))
 
 
+@pytest.mark.parametrize('shape', [(2, 7, 1000, 2, 2, 8), (2, 7, 1000, 2, 2, 24), (2, 5, 1000, 4, 2, 40), (2, 20, 1000, 2, 2, 72), (2, 10, 1000, 4, 2, 120),
+                                   (2, 40, 200, 2, 2, 24), (2, 90, 400, 2, 2, 40), (2, 40, 20, 2, 2, 24)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_an_output_gradient_that_is_not_a_number_stays_with_its_row(shape, dtype):
+    """One NaN in dO: by the formula dq of that row, dk of its key head and the NaN's own column of dv follow, and nothing
+    else changes a bit (1000 regions: every wave walks several tiles of them)."""
+    from vqa_amd import ops
+    q, k, v, do = _inputs(*shape, dtype, 21, fused=False)
+    o, saved = ops.cross_attention_fwd(q, k, v)
+    clean = ops.cross_attention_bwd(do, q, k, v, o, saved)
+    do[0, 1, 0, 3] = float('nan')
+    got = ops.cross_attention_bwd(do, q, k, v, o, saved)
+    bad = [torch.zeros_like(x, dtype=torch.bool) for x in got]
+    bad[0][0, 1, 0], bad[1][0, :, 0], bad[2][0, :, 0, 3] = True, True, True
+    for what, x, y, b in zip(('dq', 'dk', 'dv'), got, clean, bad):
+        assert bool(torch.isnan(x[b]).all()) and torch.equal(x[~b], y[~b]), what
+
+
 def test_infinite_and_nan_operands_spread_as_in_the_formula():
     from vqa_amd import ops
     q, k, v, do = _inputs(2, 3, 40, 2, 2, 16, torch.float32, 3, fused=False)

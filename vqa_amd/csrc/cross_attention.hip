@@ -808,6 +808,13 @@ __global__ void __launch_bounds__(256, waves_bwd<T>(DF, MT)) k_xattn_bwd(Args<T>
         };
         leave(a.dv, do_t, ldo, p, p_lo);
         leave(a.dk, q_t, lq, ds, ds_lo);
+        if (a.D & 8) {
+            // the result tiles wrote 8 columns behind D too: zero again, as all rows' next products run over them and a NaN
+            // of one row left there would reach every other (a guard on the stores instead: fp32 32 x 20 on 576, 43.5 -> 47 us)
+            constexpr int CH = 8 * (int)sizeof(T) / 16;
+            wave_lds_order();
+            if (lane < Y::KC * CH) *reinterpret_cast<u32x4*>(my + (lane / CH) * PITCH + a.D * (int)sizeof(T) + (lane % CH) * 16) = u32x4{};
+        }
     }
 
     float* jo = reinterpret_cast<float*>(lds);
