@@ -230,6 +230,101 @@ def test_infinite_and_nan_operands_spread_as_in_the_formula():
     assert torch.equal(bad, want)
 
 
+def _tight(q, k, v, do, kv_len=None, mask=None, scale=None):
+    """bf16 results against bounds that a factor rounded once too often breaks.
+
+    Products of bf16 values are exact in fp32.  A matrix instruction adds 32 of them (a tree of 5 additions) to its sum, and
+    a lane adds up to n / 4 numbers itself, so sums are good to F = 2^-19 of their terms' sizes over D <= 128 columns and to
+    S(n) = 2^-19 + 2^-24 n over n rows or regions.  z is good to F scale |q||k| and 2^-21 of |z| and |lse|, p to R of itself.
+    A factor in two parts is good to U = 2^-16.  Where the kernels for many rows on many regions round p once for its
+    product (W = 2^-8 of each weight), o stays a weighted mean: it moves by W sum p |v - o|, delta by W sum |ds|."""
+    B, Tq, H, D = q.shape
+    Tk, Hkv = k.shape[1], k.shape[2]
+    G = H // Hkv
+    got = _run(q, k, v, do, kv_len, mask, scale)
+    live = torch.ones(B, Tk, dtype=torch.bool, device='cuda')
+    if kv_len is not None:
+        live &= torch.arange(Tk, device='cuda')[None] < kv_len[:, None]
+    if mask is not None:
+        live &= mask
+    s = D ** -0.5 if scale is None else scale
+    leaf = [x.double().requires_grad_(True) for x in (q, k, v)]
+    o, lse = attention(*leaf, kv_len, mask, s)
+    ref = torch.autograd.grad(o, leaf, do.double())
+    o, lse = o.detach(), lse.detach()
+
+    def rows(x):
+        return x.reshape(B, Tq, Hkv, G, -1).permute(0, 2, 1, 3, 4).reshape(B, Hkv, Tq * G, -1)
+
+    def back(x):
+        return x.reshape(B, Hkv, Tq, G, D).permute(0, 2, 1, 3, 4).reshape(B, Tq, H, D)
+
+    def t(x):
+        return x.transpose(2, 3).contiguous()
+
+    Q, DO, O, L = rows(q.double()), rows(do.double()), rows(o), rows(lse.permute(0, 2, 1)[..., None])
+    K, V = (x.double().transpose(1, 2).contiguous() for x in (k, v))
+    many = Tq * G > 64 and Tk > 256
+    F, U, W = 2.0 ** -19, 2.0 ** -16, 1.01 * 2.0 ** -8 if many else 0.0
+    here = live[:, None, None, :] & torch.isfinite(L)
+
+    def S(n):
+        return 2.0 ** -19 + 2.0 ** -24 * n
+
+    z = Q @ t(K) * s
+    L = torch.where(torch.isfinite(L), L, torch.zeros_like(L))
+    p = torch.where(here, torch.exp(z - L), torch.zeros_like(z))
+    R = torch.where(here, F * abs(s) * (Q.abs() @ t(K.abs())) + 2.0 ** -21 * (2 + z.abs() + L.abs()), torch.zeros_like(z))
+    R = R + R.amax(-1, keepdim=True) + S(Tk)                                    # of p in the backward: z's error and the sum's
+    dp = DO @ t(V)
+    ds = p * (dp - (DO * O).sum(-1, keepdim=True))
+    spread = torch.cat([(p[:, :, i, :, None] * (V - O[:, :, i:i + 1]).abs()).sum(2, keepdim=True) for i in range(Tq * G)], 2)
+    base = (R * p) @ V.abs() + (U + S(Tk)) * (p @ V.abs())
+    oe = base + W * spread                                                      # of o before its rounding
+    de = (DO.abs() * (base + (U + F) * O.abs())).sum(-1, keepdim=True) + W * ds.abs().sum(-1, keepdim=True)
+    dse = p * (F * (DO.abs() @ t(V.abs())) + de) + (R + 2.0 ** -22) * ds.abs()
+    two = not many or D <= 64                                                   # dq's factor
+    lim = {'o': back(oe), 'dq': back((dse + (U if two else W) * ds.abs() + S(Tk) * ds.abs()) @ K.abs()) * abs(s),
+           'dk': (t(dse + (W or U) * ds.abs() + S(Tq * G) * ds.abs()) @ Q.abs()).transpose(1, 2) * abs(s),
+           'dv': (t(p * (R + (W or U) + S(Tq * G))) @ DO.abs()).transpose(1, 2)}
+    for what, x, r in zip(('o', 'dq', 'dk', 'dv'), (got[0], *got[2:]), (o, *ref)):
+        close(x, r, lim[what] + 1e-30, what)
+
+
+@pytest.mark.parametrize('units', [5.0, 6.5, 7.6, 7.97])
+@pytest.mark.parametrize('D', [128, 64])
+def test_one_region_above_a_lagging_maximum(units, D):
+    """More than 64 rows on more than 256 regions, nearly all weight on one late region whose score is `units` powers of two
+    above the first tile's largest, the rest 25 powers below: dO (v - o) of that region is what little the others leave."""
+    q, k, v, do = _inputs(1, 80, 300, 2, 2, D, torch.bfloat16, 41, fused=False)
+    scale = 0.125
+    k *= 0.02
+    q[..., 0] = 1
+    k[..., 0] = -25 * 0.6931 / scale
+    k[:, 3, :, 0] = 0
+    k[:, 290, :, 0] = units * 0.6931 / scale
+    _tight(q, k, v, do, scale=scale)
+
+
+@pytest.mark.parametrize('shape', [(1, 90, 400, 4, 2, 64), (1, 70, 700, 2, 2, 128), (1, 40, 2000, 2, 1, 96)])
+@pytest.mark.parametrize('sharp', [0.25, 1.0, 4.0])
+def test_weights_rounded_once_leave_a_mean(shape, sharp):
+    """The kernels for many rows on many regions, also with the regions split over workgroups: flat, ordinary and peaked
+    weights (q scaled)."""
+    q, k, v, do = _inputs(*shape, torch.bfloat16, 43, fused=False)
+    q *= sharp
+    _tight(q, k, v, do)
+
+
+def test_few_regions_count_under_many_rows():
+    """The kernels for many regions where all but a few are masked or behind the sample's count."""
+    q, k, v, do = _inputs(2, 80, 500, 2, 2, 128, torch.bfloat16, 44, fused=False)
+    _tight(q, k, v, do, kv_len=torch.tensor([3, 70], device='cuda', dtype=torch.int32))
+    mask = torch.rand(2, 500, device='cuda', generator=torch.Generator(device='cuda').manual_seed(3)) < 0.01
+    mask[:, 499] = True
+    _tight(q, k, v, do, mask=mask)
+
+
 def test_gradient_against_differences():
     """Central differences of the fp32 forward, step 1e-2: truncation 1e-4 of the gradient's norm, noise (o good to 1e-6,
     n random terms) / (2 step) about 1e-4 of it."""

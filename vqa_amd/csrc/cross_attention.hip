@@ -52,6 +52,13 @@ template <> struct Ty<bf16_t> {
         for (int i = 0; i < 4; ++i) v[i] -= bf16_to_f32((bf16_t)h[i]);
         return pack(v);
     }
+    // c + the four values
+    static __device__ __forceinline__ float sum(half h, float c) {
+        typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+        const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+        const bf16x4_t b = __builtin_bit_cast(bf16x4_t, h);
+        return __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{b[2], b[3]}, one, __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{b[0], b[1]}, one, c, false), false);
+    }
     // product over 16 (contraction), the second factor in its two parts
     static __device__ __forceinline__ f32x4 mma_parts(half a, half hi, half lo, f32x4 c) {
         c = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, lo, c, 0, 0, 0);
@@ -1346,8 +1353,9 @@ __global__ void __launch_bounds__(256) k_xattn_dkv_join(Args<T> a) {
 // 230 that the card does per byte it reads), and what feeds them is LDS: a wave that reads a 16 x 16 key fragment once for
 // two row tiles keeps LDS as busy as the matrix core.  Keys (rows, in the keys' backward) lie in LDS, two tiles of 64, for
 // eight waves of 32 rows each; the next tile is in flight in registers.  P and dS are rounded to bf16 for their products:
-// as much noise, over more than 256 terms, as the rounding of the result, sqrt(2) of its error together.  dq alone has more
-// where rows are short: its terms dS k cancel down to dS (k - k'), k' the keys' weighted mean, whose share of k is 1 / D with
+// each term moves by 2^-8 of itself at most, whatever the number of regions that count, which for terms of either sign is
+// about as much noise as the rounding of the result, sqrt(2) of its error together; in two parts they would cost half as
+// many products again.  dq alone has more where rows are short: its terms dS k cancel down to dS (k - k'), k' the keys' weighted mean, whose share of k is 1 / D with
 // independent keys, while the noise is that of dS k (1.5 of the rounding's error at D <= 32, 1.43 from 64 on).  Up to 64 its
 // dS therefore comes in two parts (8 x 509 on 2000 x 8 heads of 64: 56 us instead of 46).
 
@@ -1440,15 +1448,21 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
     };
     load(first);
     f32x4 o[MT][DT];
-    float mx[MT], sum[MT];                                   // mx: scaled, in powers of two
+    float mx[MT], sum[MT], weight[MT];                       // mx: scaled, in powers of two; sums of p, of the rounded p
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         mx[mt] = -INFINITY;
         sum[mt] = 0.f;
+        weight[mt] = 0.f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const float scale2 = positive_scale(a.scale);
+    // o is divided by the sum of the weights that its products take, p ROUNDED: it stays a weighted mean of the values, off by
+    // 2^-8 of sum p |v - o| at most, and so does the backward's delta = dO o, which is subtracted from dO v.  Divided by
+    // the sum of the exact p it would be off by up to 2^-8 of o where one region has most of the weight, however little
+    // dO (v - o) is there.  The weights' sum costs an instruction for two p (8 x 509 on 4096: 184 -> 187 us; as matrix products
+    // with ones 192).  The log-sum-exp is of the exact p.
     if (a.scale < 0.f) {
         rarely();
 #pragma unroll
@@ -1496,12 +1510,13 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, s[mt][sub][r]);
             top = groups_max(top) * scale2;
-            // the maximum follows only when a row's has grown by more than 2^8: until then p stays below 256, which
-            // costs no accuracy, and the output need not be rescaled
+            // the maximum follows only when a row's has grown by more than 2^8: until then p stays below 256 and the
+            // output need not be rescaled
             if (__any(top > mx[mt] + 8.f)) {
                 const float up = fmaxf(top, mx[mt]), at = up == -INFINITY ? 0.f : up, shrink = __builtin_amdgcn_exp2f(mx[mt] - at);
                 mx[mt] = up;
                 sum[mt] *= shrink;
+                weight[mt] *= shrink;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[mt][d] *= shrink;
             }
@@ -1519,6 +1534,8 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
             const Y::half h0[2] = {h[0], h[1]}, h1[2] = {h[2], h[3]};
             p[mt][0] = Y::join(h0);
             p[mt][1] = Y::join(h1);
+#pragma unroll
+            for (int sub = 0; sub < 4; ++sub) weight[mt] = Y::sum(h[sub], weight[mt]);
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -1539,17 +1556,18 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
     const size_t rows = (size_t)a.B * a.Hkv * a.M;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const float l = groups_sum(sum[mt]), top = mx[mt];
+        const float l = groups_sum(sum[mt]), l_rounded = groups_sum(weight[mt]), top = mx[mt];
         const int m = m0 + mt * 16 + li;
         if (m >= a.M) continue;
         const size_t at_row = (size_t)split * rows + (size_t)pair * a.M + m;
-        const float inv = a.nsplit > 1 ? 1.f : top == -INFINITY ? 0.f : 1.f / l;
+        // a key range's share of o leaves as its mean times its exact sum, which is what the join takes it for
+        const float inv = top == -INFINITY ? 0.f : (a.nsplit > 1 ? l : 1.f) / l_rounded;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int col = d * 16 + g * 4;
             if (col >= a.D) continue;
             if (a.nsplit == 1) store_out(a, row_at(a, b, hk, m) + col, o[mt][d] * inv);
-            else *reinterpret_cast<f32x4*>(a.ws + at_row * a.D + col) = o[mt][d];
+            else *reinterpret_cast<f32x4*>(a.ws + at_row * a.D + col) = o[mt][d] * inv;
         }
         if (g == 0) {
             if (a.nsplit > 1) {
