@@ -98,6 +98,31 @@ def test_strided_and_unaligned_gates():
     assert torch.equal(ops.gated_scan_fwd(wide[:, :, ::2])[0], ops.gated_scan_fwd(wide[:, :, ::2].contiguous())[0])
 
 
+@pytest.mark.parametrize('B,T,H', [(3, 24, 40), (1, 300, 8)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('size', [0.03, 1e-2, 1e-4, 1e-6])
+def test_small_states_keep_their_digits(B, T, H, dtype, size):
+    """Candidates and states of a size far below 1.  Everything is positive and the gates lie within +-2, so nothing
+    cancels and every result is good to a RELATIVE bound: a logistic or hyperbolic value to 2^-21, 1 - s(x) >= 0.12 to
+    2^-18, and each of the T steps multiplies by a forget gate (2^-21) and adds (2^-24): 2^-19 T + 2^-16 covers both directions."""
+    from vqa_amd import ops
+    g = torch.Generator(device='cuda').manual_seed(31)
+    gates = torch.randn(B, T, 4, H, device='cuda', generator=g).clamp(-2, 2)
+    gates[:, :, 2] = size * (0.5 + torch.rand(B, T, H, device='cuda', generator=g))
+    gates = gates.reshape(B, T, 4 * H).to(dtype)
+    c0 = size * (0.5 + torch.rand(B, H, device='cuda', generator=g))
+    dh = (0.5 + torch.rand(B, T, H, device='cuda', generator=g)).to(dtype)
+    dc = 0.5 + torch.rand(B, H, device='cuda', generator=g)
+    h, c, saved = ops.gated_scan_fwd(gates, None, c0)
+    dgates, dc0 = ops.gated_scan_bwd(dh, dc, gates, saved, None, c0)
+    gd, cd = gates.double().requires_grad_(True), c0.double().requires_grad_(True)
+    hr, cr = scan(gd, None, cd)
+    ref = torch.autograd.grad((hr, cr), (gd, cd), (dh.double(), dc.double()))
+    unit = 2.0 ** -19 * T + 2.0 ** -16
+    for what, x, r in (('c', c, cr), ('h', h, hr), ('dgates', dgates, ref[0]), ('dc0', dc0, ref[1])):
+        close(x, r, unit * r.detach().abs(), what)
+
+
 def test_gradient_against_differences():
     """Directional derivative of the fp32 forward by central differences.  Step e = 1e-2: the third derivative of the
     loss along a unit direction is of the order of the gradient's norm, so the truncation is below e^2 of it, and the
