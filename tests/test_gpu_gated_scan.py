@@ -98,6 +98,23 @@ def test_strided_and_unaligned_gates():
     assert torch.equal(ops.gated_scan_fwd(wide[:, :, ::2])[0], ops.gated_scan_fwd(wide[:, :, ::2].contiguous())[0])
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_strides_that_say_nothing(dtype):
+    """A size of 1 may have any stride: one step of one sample out of padded rows, one sample out of a padded batch."""
+    from vqa_amd import ops
+    H = 8
+    g = torch.Generator(device='cuda').manual_seed(6)
+    for base, take in ((torch.randn(1, 5, 4 * H + 4, device='cuda', generator=g), lambda x: x[:, 2:3, :4 * H]),
+                       (torch.randn(3, 2 * 4 * H + 4, device='cuda', generator=g), lambda x: x[:1, :2 * 4 * H].view(1, 2, 4 * H)),
+                       (torch.randn(3, 4 * H + 3, device='cuda', generator=g), lambda x: x[1:2, None, :4 * H])):
+        gates = take(base.to(dtype))
+        plain = torch.empty(gates.shape, device='cuda', dtype=dtype).copy_(gates)
+        a, b = ops.gated_scan_fwd(gates), ops.gated_scan_fwd(plain)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        for x, y in zip(ops.gated_scan_bwd(a[0], a[1], gates, a[2]), ops.gated_scan_bwd(b[0], b[1], plain, b[2])):
+            assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize('B,T,H', [(3, 24, 40), (1, 300, 8)])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('size', [0.03, 1e-2, 1e-4, 1e-6])

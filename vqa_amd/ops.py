@@ -104,10 +104,10 @@ def _scan_operands(gates, lengths, c0, name):
     _need(gates.dim() == 3 and gates.shape[2] % 32 == 0, '{}: gates must be (B, T, 4H) with H a multiple of 8', name)
     B, T, H = gates.shape[0], gates.shape[1], gates.shape[2] // 4
     sb, st, one = gates.stride()
-    if one != 1 or sb % 8 or st % 8 or (T > 1 and st < 4 * H) or sb < 0 or gates.data_ptr() % 16:
-        gates = gates.contiguous() if not gates.is_contiguous() else gates.clone()
-        sb, st, one = gates.stride()
-    st = max(st, 4 * H)
+    sb, st = sb if B > 1 else 0, st if T > 1 else 4 * H          # the stride of a size of 1 says nothing
+    if one != 1 or sb % 8 or st % 8 or st < 4 * H or sb < 0 or gates.data_ptr() % 16:
+        gates = gates.clone(memory_format=torch.contiguous_format)
+        sb, st = T * 4 * H, 4 * H
     if c0 is not None:
         _like(name, 'c0', c0, gates, (B, H), torch.float32)
         c0 = _packed(c0)
