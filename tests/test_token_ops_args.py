@@ -104,3 +104,21 @@ def test_cpu_tensors_are_refused():
     for call in (lambda: ops.gated_scan(g), lambda: ops.norm_gate(x), lambda: ops.cross_attention(q, q, q)):
         with pytest.raises(_lib.VqaHipError, match='cuda'):
             call()
+
+
+def test_scan_backward_reads_saved_states_as_they_were_saved(monkeypatch):
+    """Saved states of another type or shape are refused before any call; strided ones are packed for it."""
+    monkeypatch.setattr(ops, '_storage', lambda name, t: _lib.F32)
+    calls = []
+    monkeypatch.setattr(ops, '_call', lambda device, name, *args: calls.append(args))
+    gates, dh = torch.zeros(2, 9, 32), torch.zeros(2, 9, 8)
+    saved = torch.zeros(2, 2, 8)
+    for bad in (saved.bfloat16(), saved.half(), saved.double(), saved[:1], saved[..., :4], None):
+        with pytest.raises(ValueError, match='gated_scan'):
+            ops.gated_scan_bwd(dh, None, gates, bad)
+    assert not calls
+    wide = torch.arange(64.0).reshape(2, 2, 16)[..., ::2]                    # in place it would be read past its steps
+    ops.gated_scan_bwd(dh, None, gates, wide)
+    assert len(calls) == 1 and calls[0][7] != wide.data_ptr()
+    ops.gated_scan_bwd(dh, None, gates, saved)
+    assert calls[1][7] == saved.data_ptr()

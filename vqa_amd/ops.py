@@ -148,8 +148,9 @@ def gated_scan_bwd(dh, dc, gates, saved, lengths=None, c0=None):
         dc = _packed(dc)
     if B == 0 or T == 0 or H == 0 or (dh is None and dc is None):
         return dgates.zero_(), dc0.zero_() if dc is None else dc0.copy_(dc)
-    _need(saved is not None and tuple(saved.shape) == ((T + _SAVE - 1) // _SAVE, B, H),
-          'gated_scan: the backward needs what gated_scan_fwd(..., save=True) returned for these gates')
+    _need(saved is not None, 'gated_scan: the backward needs what gated_scan_fwd(..., save=True) returned for these gates')
+    _like('gated_scan', 'saved', saved, gates, ((T + _SAVE - 1) // _SAVE, B, H), torch.float32)
+    saved = _packed(saved)
     ws = _workspace(_floats('vqa_gated_scan_workspace_floats', B, T, H, dt), gates)
     _call(dev, 'vqa_gated_scan_bwd', _ptr(dh), _ptr(dc), gates.data_ptr(), sb, st, _ptr(lengths), _ptr(c0),
           saved.data_ptr(), dgates.data_ptr(), dc0.data_ptr(), _ptr(ws), B, T, H, dt)
