@@ -455,7 +455,7 @@ int vqa_gated_scan_bwd(const void* dh, const float* dc_last, const void* gates, 
  * regions are split over workgroups where the batch does not fill the chip.
  * Backward: d_o as o; dq as o, dk and dv (B, Tk, Hkv, D) contiguous, summed over the heads that share a key head.
  * Scores, softmax and sums are fp32.  With bf16 storage p and its gradient enter their products in two bf16 parts (good to
- * 2^-17), where matrix products are the bound (more than 64 rows per key head on more than 256 regions) rounded to bf16.
+ * 2^-16), where matrix products are the bound (more than 64 rows per key head on more than 256 regions) rounded to bf16.
  * scale is finite; D % 8 == 0, D <= VQA_CROSS_ATTN_MAX_D, B * Tq * H <= 2^27, Tk <= 2^24, Hkv * D < 2^25,
  * B * Hkv * ceil(Tq * H / Hkv / 16) <= 2^23, B * Hkv * ceil(Tk / 64) <= 2^23. */
 #define VQA_CROSS_ATTN_MAX_D 128

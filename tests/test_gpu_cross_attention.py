@@ -325,6 +325,48 @@ def test_few_regions_count_under_many_rows():
     _tight(q, k, v, do, mask=mask)
 
 
+def _formula(q, k, v, do, mask):
+    """o, dq, dk, dv product by product in 64 bits, infinities and all (regions that do not count taken out)."""
+    B, Tq, H, D = q.shape
+    G, s = H // k.shape[2], D ** -0.5
+    o, dq, dk, dv = (torch.zeros(x.shape, dtype=torch.float64, device='cuda') for x in (q, q, k, v))
+    for b in range(B):
+        at = torch.nonzero(mask[b])[:, 0]
+        for h in range(H):
+            Q, DO, K, V = (x.double() for x in (q[b, :, h], do[b, :, h], k[b, at, h // G], v[b, at, h // G]))
+            p = torch.softmax(Q @ K.t().contiguous() * s, -1)
+            o[b, :, h] = p @ V
+            ds = p * (DO @ V.t().contiguous() - (DO * o[b, :, h]).sum(-1, keepdim=True)) * s
+            dq[b, :, h] = ds @ K
+            dk[b, at, h // G] += ds.t().contiguous() @ Q
+            dv[b, at, h // G] += p.t().contiguous() @ DO
+    return o, dq, dk, dv
+
+
+@pytest.mark.parametrize('shape', [(2, 5, 90, 2, 2, 24), (1, 1, 1500, 4, 1, 64), (2, 20, 70, 2, 2, 64), (2, 40, 70, 4, 2, 40), (1, 95, 400, 2, 1, 64),
+                                   (1, 77, 300, 1, 1, 128), (2, 40, 20, 3, 1, 72)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('where', ['v', 'do'])
+def test_infinities_that_count_spread_as_in_the_formula(shape, dtype, where):
+    """+inf, -inf, NaN and finite results fall where the products of the formula put them.  Scores stay small, so no weight
+    is rounded to nothing."""
+    from vqa_amd import ops
+    q, k, v, do = _inputs(*shape, dtype, 51, fused=False)
+    mask = torch.rand(shape[0], shape[2], device='cuda', generator=torch.Generator(device='cuda').manual_seed(6)) < 0.7
+    mask[:, 5] = True
+    if where == 'v':
+        v[0, 5, 0, 2] = float('inf')
+        v[-1, 5, -1, 3] = float('-inf')
+    else:
+        do[0, -1, 0, 2] = float('inf')
+        do[-1, 0, -1, 3] = float('-inf')
+    o, saved = ops.cross_attention_fwd(q, k, v, mask=mask)
+    got = (o, *ops.cross_attention_bwd(do, q, k, v, o, saved, mask=mask))
+    for what, x, r in zip(('o', 'dq', 'dk', 'dv'), got, _formula(q, k, v, do, mask)):
+        for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(kind(x), kind(r)), (what, kind.__name__, int(kind(x).sum()), int(kind(r).sum()))
+
+
 def test_gradient_against_differences():
     """Central differences of the fp32 forward, step 1e-2: truncation 1e-4 of the gradient's norm, noise (o good to 1e-6,
     n random terms) / (2 step) about 1e-4 of it."""

@@ -46,11 +46,26 @@ template <> struct Ty<bf16_t> {
         const bf16x4_t b = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
         return __builtin_bit_cast(half, b);
     }
-    // the part of v that pack leaves behind, rounded in its turn: value = pack(v) + rest(v) to 2^-17
+    // the part of v that pack leaves behind, rounded in its turn: value = pack(v) + rest(v) to 2^-17; of an infinite v
+    // nothing is left (inf - inf would make its products NaN)
     static __device__ __forceinline__ half rest(f32x4 v, half h) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] -= bf16_to_f32((bf16_t)h[i]);
+        for (int i = 0; i < 4; ++i) {
+            v[i] -= bf16_to_f32((bf16_t)h[i]);
+            v[i] = fabsf(v[i]) < INFINITY ? v[i] : 0.f;
+        }
         return pack(v);
+    }
+    // weights >= 0 in two parts, weight = hi + lo to 2^-16: cut off, not rounded, and lo at least a number that changes
+    // nothing, so that both are above 0 where the weight is and their products with an infinite value agree
+    static __device__ __forceinline__ void split(f32x4 v, half& hi, half& lo) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned cut = __float_as_uint(v[i]) & 0xffff0000u;
+            hi[i] = (short)(cut >> 16);
+            v[i] = fmaxf(v[i] - __uint_as_float(cut), 7.888609e-31f);
+        }
+        lo = pack(v);
     }
     // c + the four values
     static __device__ __forceinline__ float sum(half h, float c) {
@@ -74,10 +89,11 @@ template <> struct Ty<bf16_t> {
         typedef s16x4_t __attribute__((address_space(3))) * lds_p;
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(lds + (row0 + (li >> 2)) * pitch + (col + 4 * (li & 3)) * 2));
     }
-    static __device__ __forceinline__ float dot(frag a, frag b) {
+    // sum a (b + c): the two parts of an output are added first, an infinite a times each could be inf - inf
+    static __device__ __forceinline__ float dot(frag a, frag b, frag c) {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += (float)a[i] * (float)b[i];
+        for (int i = 0; i < 8; ++i) s += (float)a[i] * ((float)b[i] + (float)c[i]);
         return s;
     }
 };
@@ -94,6 +110,7 @@ template <> struct Ty<float> {
     }
     static __device__ __forceinline__ half pack(f32x4 v) { return v; }
     static __device__ __forceinline__ half rest(f32x4, half) { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+    static __device__ __forceinline__ void split(f32x4 v, half& hi, half& lo) { hi = v; lo = f32x4{0.f, 0.f, 0.f, 0.f}; }
     static __device__ __forceinline__ f32x4 mma_parts(half a, half hi, half, f32x4 c) { return mma(a, hi, c); }
     static __device__ __forceinline__ frag join(const half (&h)[1]) { return h[0]; }
     static __device__ __forceinline__ half read_t(const char* lds, int pitch, int row0, int col, int li) {
@@ -102,7 +119,7 @@ template <> struct Ty<float> {
         for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float*>(lds + (row0 + i) * pitch + (col + li) * 4);
         return v;
     }
-    static __device__ __forceinline__ float dot(frag a, frag b) { return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]; }
+    static __device__ __forceinline__ float dot(frag a, frag b, frag) { return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]; }
 };
 
 // maximum / sum over the four 16-lane groups of a wave, for each l % 16, in all lanes
@@ -326,7 +343,10 @@ template <typename T> __device__ __forceinline__ void store_out(const Args<T>& a
     if constexpr (sizeof(T) == 2) {
         if (a.rest) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] -= bf16_to_f32(f32_to_bf16(v[i]));
+            for (int i = 0; i < 4; ++i) {
+                v[i] -= bf16_to_f32(f32_to_bf16(v[i]));
+                v[i] = fabsf(v[i]) < INFINITY ? v[i] : 0.f;  // (of an infinite output nothing)
+            }
             store4(a.rest + at, v);
         }
     }
@@ -456,8 +476,7 @@ __global__ void __launch_bounds__(256, waves_fwd<T>(DF, MT)) k_xattn_fwd(Args<T>
                     s[mt][ns][r] = __builtin_amdgcn_exp2f(s[mt][ns][r] * scale2 - at);
                     sum[mt] += s[mt][ns][r];
                 }
-                h[ns] = Y::pack(s[mt][ns]);
-                lo[ns] = Y::rest(s[mt][ns], h[ns]);
+                Y::split(s[mt][ns], h[ns], lo[ns]);
             }
             p[mt] = Y::join(h);
             p_lo[mt] = Y::join(lo);
@@ -653,13 +672,11 @@ __global__ void __launch_bounds__(256, waves_bwd<T>(DF, MT)) k_xattn_bwd(Args<T>
     nxt.load(a, sp, mask, len, kb, vb, (first + w0) * Y::KC, li);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        float s = 0.f, s_rest = 0.f;
+        float s = 0.f;
+        const frag none = {};
 #pragma unroll
-        for (int f = 0; f < DF; ++f) {
-            s += Y::dot(d_o[mt][f], o[mt][f]);
-            if constexpr (Y::PARTS) s_rest += Y::dot(d_o[mt][f], rest[mt][f]);
-        }
-        s = groups_sum(a.rest ? s + s_rest : s);
+        for (int f = 0; f < DF; ++f) s += Y::dot(d_o[mt][f], o[mt][f], Y::PARTS && a.rest ? rest[mt][f] : none);
+        s = groups_sum(s);
         const float l = mt * 16 + li < M ? row_lse[mt] * LOG2E : INFINITY;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -748,9 +765,8 @@ __global__ void __launch_bounds__(256, waves_bwd<T>(DF, MT)) k_xattn_bwd(Args<T>
             }
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                p[ns][mt] = Y::pack(s[ns][mt]);
+                Y::split(s[ns][mt], p[ns][mt], p_lo[ns][mt]);
                 ds[ns][mt] = Y::pack(dp[ns][mt]);
-                p_lo[ns][mt] = Y::rest(s[ns][mt], p[ns][mt]);
                 ds_lo[ns][mt] = Y::rest(dp[ns][mt], ds[ns][mt]);
             }
         }
@@ -1047,9 +1063,8 @@ __global__ void __launch_bounds__(256, 2) k_xattn_bwd_kv(Args<T> a) {
                         s[ns][r] = on ? __builtin_amdgcn_exp2f(s[ns][r] * scale2 - ls[r]) : 0.f;
                         dp[ns][r] = on ? s[ns][r] * (dp[ns][r] - de[r]) : 0.f;
                     }
-                    p[ns][qs] = Y::pack(s[ns]);
+                    Y::split(s[ns], p[ns][qs], p_lo[ns][qs]);
                     ds[ns][qs] = Y::pack(dp[ns]);
-                    p_lo[ns][qs] = Y::rest(s[ns], p[ns][qs]);
                     ds_lo[ns][qs] = Y::rest(dp[ns], ds[ns][qs]);
                 }
             }
@@ -1168,8 +1183,7 @@ __global__ void __launch_bounds__(256, 2) k_xattn_fwd_few(Args<T> a) {
                 s[n][r] = __builtin_amdgcn_exp2f(s[n][r] - at);
                 sum += s[n][r];
             }
-            hi[n] = Y::pack(s[n]);
-            lo[n] = Y::rest(s[n], hi[n]);
+            Y::split(s[n], hi[n], lo[n]);
         }
         sum = groups_sum(sum);
         const float inv = top == -INFINITY ? 0.f : 1.f / sum;
@@ -1245,15 +1259,15 @@ __global__ void __launch_bounds__(256, waves_bwd_few<T>(DF, NK)) k_xattn_bwd_few
     for (int tile = first + wave; tile < last; tile += 4) {
         const int m = tile * 16 + li;
         frag q[DF], d_o[DF];
-        float s0 = 0.f, s1 = 0.f;
+        float s0 = 0.f;
+        const frag none = {};
 #pragma unroll
         for (int f = 0; f < DF; ++f) {
             q[f] = nxt.q[f];
             d_o[f] = nxt.d_o[f];
-            s0 += Y::dot(d_o[f], nxt.o[f]);
-            if constexpr (Y::PARTS) s1 += Y::dot(d_o[f], nxt.rest[f]);
+            s0 += Y::dot(d_o[f], nxt.o[f], Y::PARTS && a.rest ? nxt.rest[f] : none);
         }
-        s0 = groups_sum(a.rest ? s0 + s1 : s0);
+        s0 = groups_sum(s0);
         const float l = m < a.M ? nxt.lse * LOG2E : INFINITY;
         fetch(tile + 4);
         wave_lds_order();
@@ -1283,9 +1297,8 @@ __global__ void __launch_bounds__(256, waves_bwd_few<T>(DF, NK)) k_xattn_bwd_few
                 s[r] = live ? __builtin_amdgcn_exp2f(s[r] * scale2 - lse[r]) : 0.f;
                 dp[r] = live ? s[r] * (dp[r] - delta[r]) * a.scale : 0.f;
             }
-            p[n] = Y::pack(s);
+            Y::split(s, p[n], p_lo[n]);
             ds[n] = Y::pack(dp);
-            p_lo[n] = Y::rest(s, p[n]);
             ds_lo[n] = Y::rest(dp, ds[n]);
             *reinterpret_cast<half*>(my_ds + (n * 16 + li) * SP + g * (int)sizeof(half)) = ds[n];
             if constexpr (Y::PARTS) *reinterpret_cast<half*>(my_ds + ((NK + n) * 16 + li) * SP + g * (int)sizeof(half)) = ds_lo[n];
@@ -1740,7 +1753,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
         Row rows[Tile::NI], stat = at_row(m_first + (lane & (R - 1)));
 #pragma unroll
         for (int i = 0; i < Tile::NI; ++i) rows[i] = at_row(m_first + (int)nxt.row(i));
-        auto load = [&]() {                                  // rows past the last one read it again; their p is zero
+        auto load = [&]() {                                  // rows past the last one read it again (cleared before their use)
 #pragma unroll
             for (int i = 0; i < Tile::NI; ++i) {
                 const int t = min(rows[i].t, a.Tq - 1), hh = rows[i].h;
@@ -1749,8 +1762,8 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
                 next(rows[i]);
             }
             const size_t at = ((size_t)b * a.H + hk * a.G + stat.h) * a.Tq + min(stat.t, a.Tq - 1);
-            const float l = a.lse[at];
-            n_delta = a.delta[at];
+            const float l = a.lse[at], de = a.delta[at];
+            n_delta = stat.t < a.Tq ? de : 0.f;
             n_lse = stat.t < a.Tq ? l * LOG2E : INFINITY;
             next(stat);
         };
@@ -1771,7 +1784,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
         int at_frag = li * PITCH + g * 16, at_t = (g * 4 + (li >> 2)) * PITCH + (li & 3) * 8;
         asm volatile("" : "+v"(at_frag), "+v"(at_t));
         int cur = 0;
-        for (int m0 = m_first; m0 < m_last; m0 += R) {
+        auto step = [&]() {
             const char* lq = lds + cur * 2 * Tile::TILE;         // q rows; dO rows a TILE behind
             const float* lst = reinterpret_cast<const float*>(lds + 4 * Tile::TILE) + cur * 2 * R;
 #pragma unroll
@@ -1818,10 +1831,20 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_bwd_kv_tile(Args<bf16_t> a) {
                     }
                 }
             }
+        };
+        int m0 = m_first;
+        for (; m0 + R <= m_last; m0 += R) {
+            step();
             cur ^= 1;
             put(cur);
             load();
             __syncthreads();
+        }
+        if (m0 < m_last) {                                   // rows past the last one: zeros (their p of 0 would make NaN of an infinite dO)
+            for (int at = (m_last - m0) * PITCH + threadIdx.x * 16; at < Tile::TILE; at += NW * 64 * 16)
+                *reinterpret_cast<u32x4*>(lds + cur * 2 * Tile::TILE + Tile::TILE + at) = u32x4{};
+            __syncthreads();
+            step();
         }
     }
 #pragma unroll
