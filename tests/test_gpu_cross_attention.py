@@ -306,6 +306,31 @@ def test_one_region_above_a_lagging_maximum(units, D):
     _tight(q, k, v, do, scale=scale)
 
 
+TIGHT = [  # B, Tq, Tk, H, Hkv, D: one row, one pass of 16 and 32 rows, few regions, two kernels, regions and rows in ranges
+    (2, 1, 300, 8, 2, 64), (1, 1, 4000, 8, 2, 128), (3, 14, 196, 4, 4, 80), (2, 20, 300, 4, 4, 40), (2, 15, 150, 6, 3, 120), (2, 40, 20, 4, 2, 72),
+    (1, 60, 9, 2, 2, 128), (2, 40, 200, 4, 2, 96), (1, 33, 700, 2, 2, 24), (1, 300, 70, 3, 1, 40)]
+
+
+@pytest.mark.parametrize('shape', TIGHT)
+@pytest.mark.parametrize('sharp', [0.25, 1.0, 4.0])
+def test_weights_and_their_gradients_keep_two_parts(shape, sharp):
+    """Everything but the kernels for many rows on many regions: no factor of a product is rounded to bf16 alone, the
+    backward's delta knows what rounding took from o."""
+    q, k, v, do = _inputs(*shape, torch.bfloat16, 43, fused=False)
+    q *= sharp
+    _tight(q, k, v, do)
+
+
+@pytest.mark.parametrize('B,Tq,Tk,H,Hkv,D', [(53, 1, 100, 17, 17, 24), (53, 5, 90, 34, 17, 40), (53, 20, 70, 17, 17, 72), (53, 40, 100, 17, 17, 64),
+                                             (53, 1, 300, 17, 17, 128), (31, 70, 60, 17, 17, 96)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_two_waves_share_a_work_item(B, Tq, Tk, H, Hkv, D, dtype):
+    """More than 512 work items, an odd number of them: two to a workgroup, the last one alone."""
+    q, k, v, do = _inputs(B, Tq, Tk, H, Hkv, D, dtype, 61)
+    kv_len = torch.randint(0, Tk + 1, (B,), device='cuda', generator=torch.Generator(device='cuda').manual_seed(7), dtype=torch.int32)
+    _check(q, k, v, do, kv_len)
+
+
 @pytest.mark.parametrize('shape', [(1, 90, 400, 4, 2, 64), (1, 70, 700, 2, 2, 128), (1, 40, 2000, 2, 1, 96)])
 @pytest.mark.parametrize('sharp', [0.25, 1.0, 4.0])
 def test_weights_rounded_once_leave_a_mean(shape, sharp):

@@ -62,6 +62,14 @@ def test_scan_and_gradients_match_64_bits(B, T, H, dtype, ragged, state):
     assert torch.equal(h, h2) and torch.equal(c, c2) and torch.equal(dgates, dg2) and torch.equal(dc0, dc02)
 
 
+@pytest.mark.parametrize('T,H', [(5000, 24), (17000, 8)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_runs_of_several_chunks(T, H, dtype):
+    """Time cut into 79 and 266 chunks: the chain's 32 runs hold up to 3 and 9 maps each."""
+    test_scan_and_gradients_match_64_bits(1, T, H, dtype, False, True)
+    test_scan_and_gradients_match_64_bits(2, T // 2, H, dtype, True, False)
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_single_steps_continue_a_sequence(dtype):
     """T = 1 calls that hand the state on against one call over all steps: the same bits for the first 8 steps, which one

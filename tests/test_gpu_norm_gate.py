@@ -78,6 +78,15 @@ def test_norm_gate_and_gradients_match_64_bits(B, T, D, dtype, gate):
     _check(*_case(B, T, D, dtype, gate, B * 1000 + T + D))
 
 
+@pytest.mark.parametrize('B,T,D', [(500, 200, 64), (1, 700000, 8), (1500, 4, 1024), (50, 50, 2400), (12, 50, 8192), (3000, 3, 64), (5000, 2, 136)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('gate', [None, 'row', 'sample', 'all'])
+def test_workgroups_walk_over_rows(B, T, D, dtype, gate):
+    """More rows than a launch holds at once, narrow and wide; several gate groups to a workgroup and several workgroups to
+    a group."""
+    _check(*_case(B, T, D, dtype, gate, 5))
+
+
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_parts_alone(dtype):
     """No weights; the norm alone; y alone; h alone."""
