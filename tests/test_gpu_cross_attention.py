@@ -350,6 +350,23 @@ def test_few_regions_count_under_many_rows():
     _tight(q, k, v, do, mask=mask)
 
 
+@pytest.mark.parametrize('shape', [(2, 5, 90, 2, 2, 24), (1, 2, 3000, 4, 1, 64), (2, 40, 70, 4, 2, 40), (1, 95, 400, 2, 1, 64), (1, 80, 2000, 2, 1, 64),
+                                   (2, 40, 20, 3, 1, 72)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_a_row_that_is_not_a_number_has_no_log_sum_exp(shape, dtype):
+    """q NaN in one row: its output and log-sum-exp are NaN (-inf says that a row attends to nothing), no other changes."""
+    from vqa_amd import ops
+    q, k, v, _ = _inputs(*shape, dtype, 52, fused=False)
+    o, (lse, _) = ops.cross_attention_fwd(q, k, v)
+    q[0, 1, -1, 3] = float('nan')
+    o2, (lse2, _) = ops.cross_attention_fwd(q, k, v)
+    bad = torch.zeros(q.shape[:3], dtype=torch.bool, device='cuda')
+    bad[0, 1, -1] = True
+    assert bool(torch.isnan(o2[bad]).all()) and torch.equal(o2[~bad], o[~bad])
+    bad = bad.transpose(1, 2)
+    assert bool(torch.isnan(lse2[bad]).all()) and torch.equal(lse2[~bad], lse[~bad])
+
+
 def _formula(q, k, v, do, mask):
     """o, dq, dk, dv product by product in 64 bits, infinities and all (regions that do not count taken out)."""
     B, Tq, H, D = q.shape

@@ -324,6 +324,10 @@ __device__ __forceinline__ float uniform(float x) { return __uint_as_float(__bui
 // needs a positive one: a negative scale turns q's sign, and of a zero the least positive number makes the same weights.
 __device__ __forceinline__ float positive_scale(float scale) { return uniform(fmaxf(fabsf(scale) * LOG2E, 1e-37f)); }
 
+// the log-sum-exp of a row from its maximum (powers of two) and its sum of 2^(score - maximum): -inf where nothing counts (an
+// empty sum), NaN where the scores are (no maximum either, but a sum that is NaN)
+__device__ __forceinline__ float log_sum(float top, float l) { return l == 0.f ? -INFINITY : (top + log2f(l)) * LN2; }
+
 // keeps a uniform branch a branch: the compiler would select, element by element, on every pass
 __device__ __forceinline__ void rarely() { asm volatile(""); }
 
@@ -526,7 +530,7 @@ __global__ void __launch_bounds__(256, waves_fwd<T>(DF, MT)) k_xattn_fwd(Args<T>
                 float* st = a.ws + ((size_t)a.nsplit * rows * a.D + (row0 + it) * 2);
                 st[0] = top;
                 st[1] = l;
-            } else if (a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(l)) * LN2;
+            } else if (a.lse) a.lse[stat_at(a, b, hk, m)] = log_sum(top, l);
         }
     }
     float* jo = reinterpret_cast<float*>(lds);
@@ -571,7 +575,7 @@ __global__ void __launch_bounds__(256) k_xattn_join(Args<T> a) {
         v += w * *reinterpret_cast<const f32x4*>(a.ws + (s * rows + row) * a.D + col);
     }
     store_out(a, row_at(a, b, hk, m) + col, v * (top == -INFINITY ? 0.f : 1.f / l));
-    if (col == 0 && a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(l)) * LN2;
+    if (col == 0 && a.lse) a.lse[stat_at(a, b, hk, m)] = log_sum(top, l);
 }
 
 // ---- backward -------------------------------------------------------------------------------
@@ -1197,7 +1201,7 @@ __global__ void __launch_bounds__(256, 2) k_xattn_fwd_few(Args<T> a) {
             const int col = d * 16 + g * 4;
             if (m < a.M && col < a.D) store_out(a, at_row + col, o * inv);
         }
-        if (g == 0 && m < a.M && a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * LN2;
+        if (g == 0 && m < a.M && a.lse) a.lse[stat_at(a, b, hk, m)] = log_sum(top, sum);
     }
 }
 
@@ -1587,7 +1591,7 @@ __global__ void __launch_bounds__(NW * 64) k_xattn_fwd_tile(Args<bf16_t> a) {
                 float* st = a.ws + (size_t)a.nsplit * rows * a.D + at_row * 2;
                 st[0] = top;
                 st[1] = l;
-            } else if (a.lse) a.lse[stat_at(a, b, hk, m)] = top == -INFINITY ? -INFINITY : (top + log2f(l)) * LN2;
+            } else if (a.lse) a.lse[stat_at(a, b, hk, m)] = log_sum(top, l);
         }
     }
 }
