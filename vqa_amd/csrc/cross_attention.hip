@@ -1919,13 +1919,18 @@ int bwd_splits(int B, int Tq, int Tk, int H, int Hkv, int dtype) { return key_sp
 
 // Waves per work item: two, so that an item's end (the join) and the next one's beginning overlap with other items (64 x 8
 // rows on 700 x 8 heads: 17 against 21 us); four where the items are fewer than two to a CU and only their own length counts
-// (one image of 196 regions: 5.6 against 7.2), and where two would fill a last round of CUs by less than half (150 x 1 row
-// on 1000 x 8 heads of 128, fp32: 229 against 243 forward, 440 against 493 backward; 40 x 60 on 700: 50 against 64), if an item is
-// `least` tiles long.
+// (one image of 196 regions: 5.6 against 7.2), and where two would fill a last round of CUs (512 items) by less than half, if
+// an item is `least` tiles long.  Time with four over time with two, 520 - 4100 items, both types, widths 64 and 128:
+//   one row tile a wave, forward, last round less than half full: 0.87 - 1.04 from 5 tiles on, 0.85 - 0.97 from 16; others 0.96 -
+//     1.10 from 16, up to 1.2 below; one-pass backward: 0.85 - 1.03 and 0.84 - 0.97, others 0.91 - 1.11, below 9 tiles up to 1.5;
+//   several row tiles a wave, forward: 1.0 - 1.25 below 16 tiles, 0.88 - 1.07 from 16 on, others 0.95 - 1.17; dq with dk, dv the
+//     same to a third of it: 0.93 - 1.05 from 16 tiles on;
+//   from the sixth round on (2816 items) nothing is left to gain: 0.94 - 1.04.
 int waves_of(const int items, const int tiles, const int least) {
     return items < 512 || (tiles >= least && (items - 1) % 512 < 256 && items <= 2816) ? 4 : 2;
 }
-constexpr int LEAST_FWD = 5, LEAST_BWD = 9, LEAST_Q = 16;     // forward, one-pass backward, dq of many rows
+constexpr int least_fwd(int row_tiles) { return row_tiles == 1 ? 5 : 16; }
+constexpr int LEAST_BWD = 9, LEAST_Q = 16;                    // one-pass backward, dq of many rows
 
 // The two-kernel backward: blocks, key ranges of the dq kernel, row ranges of the dk / dv kernel.  Ranges only where the
 // blocks alone leave CUs idle; row ranges of at least 4 tiles, at most 16 (slabs of dk and dv are as large as they are).
@@ -1954,7 +1959,7 @@ TwoPlan two_plan(int B, int Hkv, long M, int Tk, int D, int dtype) {
 
 template <typename T, int DF, int MT> void launch_fwd(const Args<T>& a, hipStream_t s) {
     const int grid = 8 * ((a.blocks + 7) / 8);
-    if (waves_of(a.items, a.tiles_split, LEAST_FWD) == 2) k_xattn_fwd<T, DF, MT, 2><<<grid, 256, 0, s>>>(a);
+    if (waves_of(a.items, a.tiles_split, least_fwd(MT)) == 2) k_xattn_fwd<T, DF, MT, 2><<<grid, 256, 0, s>>>(a);
     else k_xattn_fwd<T, DF, MT, 4><<<grid, 256, 0, s>>>(a);
 }
 template <typename T, int DF> void launch_fwd_mt(const Args<T>& a, int mt, hipStream_t s) {
@@ -2058,7 +2063,7 @@ int fwd(Args<T> a, int nsplit, int dtype, hipStream_t stream) {
         const int tiles = (a.Tk + Ty<T>::KC - 1) / Ty<T>::KC;
         a.tiles_split = (tiles + nsplit - 1) / nsplit;
         a.items = a.B * a.Hkv * a.row_blocks * nsplit;
-        a.blocks = waves_of(a.items, a.tiles_split, LEAST_FWD) == 2 ? (a.items + 1) / 2 : a.items;
+        a.blocks = waves_of(a.items, a.tiles_split, least_fwd(mt)) == 2 ? (a.items + 1) / 2 : a.items;
         BY_WIDTH(T, a.D, (launch_fwd_mt<T, DF>(a, mt, stream)));
     }
     int rc = vqa_check_launch("vqa_cross_attn_fwd");
