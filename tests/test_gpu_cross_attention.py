@@ -163,6 +163,21 @@ def test_strides_scale_and_sharp_scores():
     _check(q, k, v, do)
 
 
+@pytest.mark.parametrize('shape', [(3, 7, 90, 2, 2, 64), (3, 40, 70, 4, 2, 64), (3, 90, 400, 2, 2, 64), (3, 40, 20, 3, 1, 64), (3, 5, 1, 2, 1, 24)])
+def test_masks_of_any_layout(shape):
+    """One mask for all samples (stride 0), a slice of a wider one, every second byte of one, numbers other than 1; counts in
+    64 bits, below zero and past the regions."""
+    q, k, v, do = _inputs(*shape, torch.bfloat16, 13)
+    Tk, g = shape[2], torch.Generator(device='cuda').manual_seed(8)
+    wide = torch.rand(3, 2 * Tk + 3, device='cuda', generator=g) < 0.6
+    kv_len = torch.tensor([2 ** 40, -5, (Tk + 1) // 2], device='cuda')
+    for mask in (wide[:1, :Tk].expand(3, -1), wide[:, 3:3 + Tk], wide[:, 1:2 * Tk:2], wide[:, :Tk].to(torch.uint8) * 6):
+        for n in (None, kv_len):
+            plain = torch.empty(mask.shape, dtype=torch.bool, device='cuda').copy_(mask != 0)
+            for a, b in zip(_run(q, k, v, do, n, mask), _run(q, k, v, do, None if n is None else n.clamp(0, Tk).int(), plain)):
+                assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize('shape', [(2, 7, 90, 2, 2, 64), (1, 40, 70, 4, 2, 64), (2, 90, 400, 2, 2, 64), (2, 40, 20, 3, 1, 64)])
 @pytest.mark.parametrize('scale', [0.6, -0.6, 0.0, -1e-3])
 def test_scores_far_below_zero_and_signs_of_the_scale(shape, scale):
