@@ -420,8 +420,8 @@ int vqa_cast_pad(const float* src, int ld_src, void* dst, int ld_dst, int M, int
  *   c_t = s(f_t) c_{t-1} + s(i_t) tanh(g_t),  h_t = s(o_t) tanh(c_t)        (s: the logistic function)
  *   gates    (B, T) rows of 4H, gate order i, f, g, o, row (b, t) at gates + b * sb + t * st (elements, multiples of 8,
  *            st >= 4H)
- *   lengths  optional (B): sample b has lengths[b] steps (clamped to [0, T]); behind them the state stays, h is 0, the
- *            gates are not read and their gradient is 0
+ *   lengths  optional (B): sample b has lengths[b] steps (clamped to [0, T]); behind them the state stays and h is 0, what
+ *            the gates hold has no effect and their gradient is 0
  *   c0       optional (B, H) fp32 starting state (0 when NULL); c_last optional (B, H) fp32: the state after the last
  *            step, so that a call with T = 1 is one step of a running sequence
  *   h        (B, T, H)
@@ -449,13 +449,17 @@ int vqa_gated_scan_bwd(const void* dh, const float* dc_last, const void* gates, 
  *   o           (B, Tq, H, D) contiguous; a row with no region that counts is 0
  *   o_rest      bf16 storage only, as o: what rounding took from o, for the backward (its sums of dO o are subtracted from
  *               dO v, and with few regions, or one that has most of the weight, little is left of either); may be NULL
- *   lse         (B, H, Tq) fp32 log-sum-exp of a row's scores (-inf for such a row), for the backward; may be NULL
+ *   lse         (B, H, Tq) fp32 log-sum-exp of a row's scores (-inf for such a row, NaN where they are), for the backward;
+ *               may be NULL
  *   workspace   vqa_cross_attn_{fwd,bwd}_workspace_floats fp32 (may be 0: NULL), scratch of one call
  * One query row against many regions (serving) is Tq = 1: the H / Hkv heads of a key head share one reading of it, and the
  * regions are split over workgroups where the batch does not fill the chip.
  * Backward: d_o as o; dq as o, dk and dv (B, Tk, Hkv, D) contiguous, summed over the heads that share a key head.
  * Scores, softmax and sums are fp32.  With bf16 storage p and its gradient enter their products in two bf16 parts (good to
- * 2^-16), where matrix products are the bound (more than 64 rows per key head on more than 256 regions) rounded to bf16.
+ * 2^-16); where matrix products are the bound (more than 64 rows per key head on more than 256 regions) they are rounded to
+ * bf16 once, except dq's from D <= 64: o is then a mean of the values with weights good to 2^-8, a gradient's terms are.
+ * The backward recomputes p from lse, which is good to 2^-22 of the score's size: scores (scale q.k) are meant to stay below
+ * 2^12 or so, where that is a quarter of a bf16 half step; past 2^20 p is lost to it, past 2^28 results may be NaN.
  * scale is finite; D % 8 == 0, D <= VQA_CROSS_ATTN_MAX_D, B * Tq * H <= 2^27, Tk <= 2^24, Hkv * D < 2^25,
  * B * Hkv * ceil(Tq * H / Hkv / 16) <= 2^23, B * Hkv * ceil(Tk / 64) <= 2^23. */
 #define VQA_CROSS_ATTN_MAX_D 128

@@ -13,12 +13,13 @@
 // the other operand is read from LDS in that key order, transposed by ds_read_b64_tr_b16 for bf16.
 //
 // With few rows per key head the bound is HBM: K and V are read once (backward: and dK, dV written once).  Measured, bf16:
-//   64 x 1 row x 8 key heads of 128 (4 query heads each) on 4096 regions, ragged: 155 us, at the copy rate (5.1 TB/s)
-//   256 x 14 on 196 x 15 heads of 80, ragged: forward 55 - 65 us, backward 97 - 103 us
+//   64 x 1 row x 8 key heads of 128 (4 query heads each) on 4096 regions, ragged: 156 us, at the copy rate (5.1 TB/s)
+//   256 x 14 on 196 x 15 heads of 80, ragged: forward 62 us, backward 105 us
 // with many rows and regions the matrix cores:
-//   8 x 509 on 4096 x 8 key heads of 128 (2 each): forward 163 us (840 TFLOP/s), dq 201 us (three products, 1020 TFLOP/s),
-//   dk and dv 321 us (four products, 850 TFLOP/s); a large library product reaches 1180 there
-// and fp32 32 x 20 on 576 x 8 heads of 64: 21 and 42 us.  The variants, by rules of two_plan(), few(), one_pass(), tiled():
+//   8 x 509 on 4096 x 8 key heads of 128 (2 each): forward 172 us (790 TFLOP/s), dq 208 us (three products, 990 TFLOP/s),
+//   dk and dv 325 us (four products, 840 TFLOP/s), delta 11; a large library product reaches 1180 there
+// and fp32 32 x 20 on 576 x 8 heads of 64: 22 and 44 us (medians under the profiler, whose short runs clock lower: these
+// kernels take 3 - 12 % less in passes back to back).  The variants, by rules of two_plan(), few(), one_pass(), tiled():
 // k_xattn_fwd / k_xattn_bwd stream the keys past up to 64 (32) rows in registers; k_xattn_bwd_q / _bwd_kv for more rows;
 // k_xattn_*_tile for more than 64 rows on more than 256 keys; k_xattn_*_few for at most 32 keys.
 #include "common.h"

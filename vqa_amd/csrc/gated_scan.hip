@@ -2,16 +2,17 @@
 //   c_t = s(f_t) c_{t-1} + s(i_t) tanh(g_t),   h_t = s(o_t) tanh(c_t)          (s: the logistic function)
 // over gate rows of 4H in the order i, f, g, o, each sample for its own number of steps.  The recurrence is linear in c,
 // so a stretch of steps acts on the state it starts from as x -> P x + C with P the product of its forget gates.
-// The work is bound by HBM (forward: 4 gates read, h written; backward: 4 gates and dh read, 4 gradients written), and
-// the gates are to be read ONCE: a workgroup takes 64 V neighbouring units and a block of 8 steps per wave, every wave
+// The bound is HBM (forward: 4 gates read, h written; backward: 4 gates and dh read, 4 gradients written), with the
+// arithmetic close behind, and the gates are to be read ONCE: a workgroup takes 64 V neighbouring units and a block of 8 steps per wave, every wave
 // reads its 8 steps into registers and folds them, the waves' maps are chained through LDS, and every wave then walks its
 // steps again from its true starting state, out of registers, while the next block is on its way.  Only where the units of
 // all samples together make too few workgroups is time itself cut into chunks for different workgroups; the maps of the
 // chunks then take a pass over the gates of their own (with an atomic-free chain between the passes).
-// Measured (bf16): 256 x 14 steps of 2400 units, ragged, 17 us forward and 31 backward; 1 x 16001 steps of 2048 units, cut
-// into 251 chunks, 50 (maps) + 57 us forward, 3.9 and 5.7 TB/s, and 80 + 129 us backward, 4.1 and 4.6 TB/s, where a large
-// copy reaches 5.1; 7 x 577 steps of 1200 units, fp32, 27 and 44 us.  At ten transcendental instructions a step and unit the
-// arithmetic takes about half of that.  Sixteen waves to a workgroup (half the blocks) made the backward spill, narrower
+// Measured (bf16, medians under the profiler): 256 x 14 steps of 2400 units, ragged, 19 us forward and 34 backward; 1 x 16001
+// steps of 2048 units, cut into 251 chunks, 52 (maps) + 72 us forward, 3.8 and 4.6 TB/s, and 87 + 152 us backward, 3.8 and
+// 3.9 TB/s, where a large copy reaches 5.1; 7 x 577 steps of 1200 units, fp32, 28 - 32 and 41 - 46 us.  About sixty vector
+// instructions a step and unit, ten of them transcendental, keep the vector units busy 97 % of the long forward walk's
+// time, 67 - 77 % of its other passes', 51 and 64 % at 256 x 14, 23 and 30 % at 7 x 577.  Sixteen waves to a workgroup (half the blocks) made the backward spill, narrower
 // tiles of units with more shares of steps per wave gained nothing.
 #include "common.h"
 #include "vqa_hip.h"
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(MOST_WAVES * 64) k_scan_bwd(Args<T> a) {
 
 // Chunks of time: one where the units make 96 workgroups (which read as fast as the card does, one to a CU) or the sequence
 // is a few blocks long; otherwise chunks of one block, which a workgroup's eight waves take at once (8 x as many single
-// waves that each walk 64 steps: 358 against 338 us for 16001 steps of 2048 units, forward and backward).
+// waves that each walk 64 steps: 6 % more for 16001 steps of 2048 units, forward and backward).
 int chunk_of(int B, int T_, int H, int dtype) {
     const int v = dtype == VQA_BF16 ? 2 : 1, block = MOST_WAVES * SAVE;
     const long tiles = ((long)B * (H / v) + 63) / 64;

@@ -10,9 +10,9 @@
 // row they would be more L2 traffic than the row itself); the backward, which needs them beside five operands and three
 // running column sums, keeps them in LDS instead (in registers it spilled).  Column sums leave a workgroup as one slab row
 // and a second kernel adds the slabs in order.
-// Measured (a large copy reaches 5.1 TB/s): 100352 rows of 2048, bf16, a gate row per 196: forward 352 us (4.7 TB/s),
-// backward 517 + 15 us (4.8 TB/s); 3570 rows of 2400, fp32, a gate per row: 46 us (3.7 TB/s) and 66 + 5 us (4.1 TB/s);
-// 14 rows of 1200: 4.5 us.
+// Measured (a large copy reaches 5.1 TB/s): 100352 rows of 2048, bf16, a gate row per 196: forward 364 us (4.5 TB/s),
+// backward 517 + 15 us (4.8 TB/s); 3570 rows of 2400, fp32, a gate per row: 47 us (3.7 TB/s) and 67 + 5 us (4.1 TB/s);
+// 14 rows of 1200: 4.7 us.
 #include "common.h"
 #include "vqa_hip.h"
 
@@ -20,7 +20,7 @@ namespace {
 
 constexpr int MAX_D = 8192;                  // 1024 threads x 8 columns
 
-// Teams of a workgroup for width D; rows_min: no more teams than this.
+// Teams of a workgroup for width D; rows_max: no more teams than this.
 struct Team { int lanes, teams; };
 Team team_of(int D, long rows_max) {
     const int v = D / 8;

@@ -7,8 +7,9 @@ no counterpart.)
 
 Each operator comes as a differentiable function and as the explicit pair ``*_fwd`` / ``*_bwd`` it is made of, for
 training loops that keep their own buffers.  Tensors live on one HIP device; the work goes to torch's current stream of
-THAT device, whichever device is current.  Storage is float32 or bfloat16, arithmetic float32.  An operand whose rows
-the kernels cannot read in 16-byte pieces (odd strides or addresses) is copied first.  Outputs are new tensors.
+THAT device, whichever device is current.  Storage is float32 or bfloat16, arithmetic float32 (the factors that attention's
+matrix products take in bfloat16 are named in include/vqa_hip.h).  An operand whose rows the kernels cannot read in 16-byte
+pieces (odd strides or addresses) is copied first.  Outputs are new tensors.
 """
 from __future__ import annotations
 
